@@ -27,6 +27,7 @@ HCP_SRC_NONE, HCP_SRC_A, HCP_SRC_B, HCP_SRC_PAGED, HCP_SRC_LIST = 0, 1, 2, 3, 4
 HCP_SRC_EXT0 = 16          # HCP_SRC_EXT0 + i: extra contiguous source i
 HCP_MAX_ITEM_SEGMENTS = 8  # segments in one work item's list
 HCP_MAX_EXT_SOURCES = 8    # extra contiguous sources per call
+HCP_ROPE_CACHE_NONE, HCP_ROPE_CACHE_SAME, HCP_ROPE_CACHE_Q4 = 0, 1, 2
 
 
 class HcpKvSource(ctypes.Structure):
@@ -126,6 +127,54 @@ class HcpDecodeArgs(ctypes.Structure):
     ]
 
 
+class HcpStepPlanArgs(ctypes.Structure):
+    _fields_ = [
+        ("context_lens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p), ("pos_base", ctypes.c_void_p),
+        ("block_table", ctypes.c_void_p), ("block_table_stride", ctypes.c_int64),
+        ("block_table_width", ctypes.c_int64),
+        ("free_blocks", ctypes.c_void_p), ("num_free", ctypes.c_int64), ("free_head", ctypes.c_void_p),
+        ("query_start", ctypes.c_void_p), ("seq_lens", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p), ("token_req", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+        ("free_head_out", ctypes.c_void_p), ("missing_out", ctypes.c_void_p),
+        ("num_reqs", ctypes.c_int32), ("block_size", ctypes.c_int32), ("num_tokens", ctypes.c_int64),
+    ]
+
+
+class HcpNormRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_row_stride", ctypes.c_int64),
+        ("k", ctypes.c_void_p), ("k_row_stride", ctypes.c_int64),
+        ("v", ctypes.c_void_p), ("v_row_stride", ctypes.c_int64),
+        ("q_out", ctypes.c_void_p), ("q_out_row_stride", ctypes.c_int64),
+        ("k_out", ctypes.c_void_p), ("k_out_row_stride", ctypes.c_int64),
+        ("positions", ctypes.c_void_p), ("num_tokens", ctypes.c_int64),
+        ("cos_sin", ctypes.c_void_p), ("table_rows", ctypes.c_int64), ("table_stride", ctypes.c_int64),
+        ("table_dtype", ctypes.c_int32), ("rotary", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("q_weight", ctypes.c_void_p), ("k_weight", ctypes.c_void_p),
+        ("kv_cache", ctypes.c_void_p), ("slot_mapping", ctypes.c_void_p), ("num_blocks", ctypes.c_int64),
+        ("block_size", ctypes.c_int32), ("cache_kind", ctypes.c_int32),
+    ]
+
+
+class HcpDecodeQ4Args(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("scale", ctypes.c_float), ("block_size", ctypes.c_int32),
+        ("q", ctypes.c_void_p), ("q_rows", ctypes.c_int64), ("q_row_stride", ctypes.c_int64),
+        ("kv_cache", ctypes.c_void_p), ("num_blocks", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p), ("block_table_rows", ctypes.c_int64),
+        ("block_table_stride", ctypes.c_int64), ("block_table_width", ctypes.c_int64),
+        ("kv_lens", ctypes.c_void_p), ("token_req", ctypes.c_void_p),
+        ("out", ctypes.c_void_p), ("out_row_stride", ctypes.c_int64), ("out_dtype", ctypes.c_int32),
+        ("_pad0", ctypes.c_int32),
+        ("lse", ctypes.c_void_p), ("lse_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 # Every C entry point with its ctypes signature.  ``tests`` check that the
 # built library exports exactly the names ``include/hcp_ring.h`` declares.
 SIGNATURES = {
@@ -147,6 +196,18 @@ SIGNATURES = {
         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
         ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
         ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p]),
+    "hcp_kv_plan_step": (ctypes.c_int, [ctypes.POINTER(HcpStepPlanArgs), ctypes.c_void_p]),
+    "hcp_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(HcpNormRopeArgs), ctypes.c_void_p]),
+    "hcp_kv_cache_update_q4": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
+        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+        ctypes.c_int32, ctypes.c_int32, ctypes.c_void_p]),
+    "hcp_kv_cache_gather_q4": (ctypes.c_int, [
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32,
+        ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+        ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p]),
+    "hcp_decode_q4_splitkv": (ctypes.c_int, [ctypes.POINTER(HcpDecodeQ4Args), ctypes.c_void_p]),
+    "hcp_decode_q4_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(HcpDecodeQ4Args)]),
     "hcp_ipc_export": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.POINTER(ctypes.c_int64)]),
     "hcp_ipc_open": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int32, ctypes.POINTER(ctypes.c_void_p)]),
     "hcp_ipc_close": (ctypes.c_int, [ctypes.c_void_p]),

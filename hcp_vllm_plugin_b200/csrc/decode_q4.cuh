@@ -1,0 +1,528 @@
+// Single-token attention over the 4-bit paged cache (q4_cache.cuh) for B200.
+//
+// For every query row r with its request's pages and n = kv_lens[r] keys, per
+// head h of KV head h / G:
+//   o = sum_j softmax_j(scale q . k_j) v_j,   k_j, v_j = lo + s n  per 64 dims,
+//   lse = log sum_j exp(scale q . k_j).
+//
+// Bound by HBM: 9/8 D bytes per key and KV head (K and V), against 2 G D
+// products.  What has to be kept small is the work per byte.  So:
+//   * the whole numbers n are the matrix operands, exact in 16 bits; scales and
+//     lowest values are applied outside, per 64-dim group:
+//       q . k  = sum_g  s_g (q_g . (n_g - 8)) + (lo_g + 8 s_g) sum(q_g)
+//       o_g    = sum_j (p_j s_j) (n_j - 8)    + sum_j p_j (lo_j + 8 s_j)
+//     (n - 8 keeps the accumulated sums as small as the result's own terms);
+//   * keys are the rows of the first product (16 keys x 8 heads) and dims those of
+//     the second (16 dims x 8 heads), so a group of up to 8 query heads fills the
+//     instruction's 8 columns instead of half of 16 rows;
+//   * the tile layout gives every lane its fragments of both products in whole
+//     16-byte pieces: no shared memory, no transposes; only the 8 x 8 blocks of P
+//     are transposed between the products (movmatrix);
+//   * p_j s_j enters the second product as a bf16 high part and the rest (two
+//     products), ~16 significant bits; bf16 whatever the rows' type, for its range.
+//
+// Split: all rows' tiles of 16 keys, heads outermost in a row, form one line that
+// the blocks cut into equal pieces, so any mix of lengths is even and nothing
+// about the lengths has to be known on the host.  Every block sums the lengths
+// itself.  A (row, KV head) that lies inside one piece is written to out by its
+// block; one that is cut leaves a partial (O, m, l) per piece in the workspace, and
+// a second kernel, already resident when the first ends, joins them in order.
+// Inside a piece the four warps take the tiles in turn and join in shared memory.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "decode.cuh"
+#include "q4_cache.cuh"
+
+namespace hcp {
+
+constexpr int kDq4Warps = 4;
+constexpr int kDq4Threads = kDq4Warps * 32;
+constexpr int kDq4CtasPerSm = 3;
+constexpr int kDq4Sms = 148;
+constexpr int kDq4Ctas = kDq4Sms * kDq4CtasPerSm;
+constexpr int kDq4MinTiles = kDq4Warps;  // tiles of a piece at least: one a warp
+
+struct DecodeQ4Params {
+  const void* q;
+  long long q_row_stride;
+  const uint8_t* cache;
+  const int32_t* block_table;
+  long long bt_stride;
+  long long bt_width;
+  long long bt_rows;
+  long long num_blocks;
+  const int32_t* kv_lens;
+  const int32_t* token_req;   // may be null: row r reads table row r
+  void* out;
+  long long out_row_stride;
+  float* lse;                 // may be null
+  long long lse_stride;
+  int4* desc;                 // [ctas] {row, kv head, slot of the first part, parts}; row -1: none
+  float2* part_ml;            // [ctas][2][G] base (log2 units) and sum
+  float* part_o;              // [ctas][2][G][D] sums to that base
+  int rows;
+  int num_heads;
+  int num_kv_heads;
+  int group;
+  int block_size;
+  int sub_shift;              // log2(tiles in a block)
+  float scale_log2;
+  int out_dt;
+};
+
+__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ldg_stream2(const uint8_t* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// Nibbles I and I+4 of a word as a pair n - 8 in 16 bits: with the nibble in the
+// low mantissa bits of 128 (bf16) or 1024 (fp16) the value is 128 + n or 1024 + n,
+// and the subtraction is exact.
+template <bool F16, int I>
+__device__ __forceinline__ uint32_t q4_pair(uint32_t w) {
+  constexpr uint32_t kBase = F16 ? 0x64006400u : 0x43004300u;
+  const uint32_t v = ((w >> (4 * I)) & 0x000f000fu) | kBase;
+  if constexpr (F16) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __floats2half2_rn(1032.f, 1032.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(136.f, 136.f));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+}
+
+// A lane's share of one tile: K rows of tokens 2g and 2g+1, V pieces, parameters
+// of both tokens.
+template <int D>
+struct Q4Frag {
+  uint32_t k[2][4 * Q4<D>::kGroups / 2];  // D = 128: 4 words a token; 64: 2
+  uint32_t v[Q4<D>::kGroups][4];
+  uint32_t prm[2][2 * Q4<D>::kGroups];    // per token: K (s, lo) of each group, then V
+};
+
+template <int D>
+__device__ __forceinline__ void q4_load(Q4Frag<D>& f, const uint8_t* tile, int g, int t) {
+  using L = Q4<D>;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint8_t* kp = tile + (2 * g + e) * (D / 2) + t * (D / 8);
+    const uint8_t* pp = tile + L::kParamOff + (2 * g + e) * L::kTokenParams;
+    if constexpr (D == 128) {
+      const uint4 a = ldg_stream(kp), b = ldg_stream(pp);
+      f.k[e][0] = a.x; f.k[e][1] = a.y; f.k[e][2] = a.z; f.k[e][3] = a.w;
+      f.prm[e][0] = b.x; f.prm[e][1] = b.y; f.prm[e][2] = b.z; f.prm[e][3] = b.w;
+    } else {
+      const uint2 a = ldg_stream2(kp), b = ldg_stream2(pp);
+      f.k[e][0] = a.x; f.k[e][1] = a.y;
+      f.prm[e][0] = b.x; f.prm[e][1] = b.y;
+    }
+  }
+#pragma unroll
+  for (int hf = 0; hf < L::kGroups; ++hf) {
+    const uint4 a = ldg_stream(tile + L::kVOff + (hf * 8 + g) * 64 + t * 16);
+    f.v[hf][0] = a.x; f.v[hf][1] = a.y; f.v[hf][2] = a.z; f.v[hf][3] = a.w;
+  }
+}
+
+// Tiles of a row (0 for a padding row or an empty one).
+__device__ __forceinline__ int dq4_len(const DecodeQ4Params& p, int r, int& req) {
+  req = p.token_req != nullptr ? p.token_req[r] : r;
+  if (req < 0 || req >= p.bt_rows) return -1;
+  const long long n = max(0, p.kv_lens[r]);
+  return static_cast<int>(min(n, p.bt_width * p.block_size));
+}
+__device__ __forceinline__ int dq4_tiles(int len) { return len > 0 ? (len + 15) >> 4 : 0; }
+
+template <int D, int NT>
+struct Dq4Smem {
+  static constexpr int kCols = 8 * NT;
+  static constexpr int kPitch = D + 4;
+  float o[kDq4Warps][kCols][kPitch];
+  float m[kDq4Warps][kCols];
+  float l[kDq4Warps][kCols];
+  long long start[kDq4Threads + 1];
+  long long wsum[kDq4Warps];
+};
+
+__device__ __forceinline__ void dq4_store(const DecodeQ4Params& p, long long row, int head, int D, int d, float v) {
+  const long long i = row * p.out_row_stride + static_cast<long long>(head) * D + d;
+  if (p.out_dt == HCP_F32) static_cast<float*>(p.out)[i] = v;
+  else if (p.out_dt == HCP_F16) static_cast<__half*>(p.out)[i] = __float2half_rn(v);
+  else static_cast<__nv_bfloat16*>(p.out)[i] = __float2bfloat16_rn(v);
+}
+
+template <int D, bool F16, int NT>
+__global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
+    decode_q4_kernel(const __grid_constant__ DecodeQ4Params p) {
+  using L = Q4<D>;
+  constexpr int NG = L::kGroups;
+  constexpr int KW = 2 * NG;           // K words of a lane and token
+  __shared__ Dq4Smem<D, NT> sm;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, t = lane & 3;
+  const int G = p.group, Hkv = p.num_kv_heads;
+
+  // ---- the line of tiles: sums of every thread's run of rows
+  const int run = (p.rows + kDq4Threads - 1) / kDq4Threads;
+  long long mine = 0;
+  for (int r = tid * run; r < min(p.rows, (tid + 1) * run); ++r) {
+    int req;
+    mine += dq4_tiles(dq4_len(p, r, req));
+  }
+  long long inc = mine;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const long long a = __shfl_up_sync(0xffffffffu, inc, s);
+    if (lane >= s) inc += a;
+  }
+  if (lane == 31) sm.wsum[warp] = inc;
+  __syncthreads();
+  long long before = 0;
+  for (int w = 0; w < warp; ++w) before += sm.wsum[w];
+  sm.start[tid] = before + inc - mine;
+  if (tid == kDq4Threads - 1) sm.start[kDq4Threads] = before + inc;
+  __syncthreads();
+  const long long total = sm.start[kDq4Threads] * Hkv;
+  const long long piece = max(static_cast<long long>(kDq4MinTiles), (total + gridDim.x - 1) / gridDim.x);
+  long long f = blockIdx.x * piece;
+  const long long f_end = min(total, f + piece);
+  const long long f_begin = f;
+
+  // rows without keys: zeros, lse -inf
+  for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+    int req;
+    if (dq4_len(p, r, req) != 0) continue;
+    for (int e = tid; e < p.num_heads * D; e += kDq4Threads) dq4_store(p, r, e / D, D, e % D, 0.f);
+    if (p.lse != nullptr)
+      for (int h = tid; h < p.num_heads; h += kDq4Threads) p.lse[h * p.lse_stride + r] = -INFINITY;
+  }
+  int4 desc = make_int4(-1, 0, 0, 0);
+  if (f < f_end) {
+    // the row that holds tile f
+    int lo = 0, hi = kDq4Threads - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (sm.start[mid] * Hkv <= f) lo = mid; else hi = mid - 1;
+    }
+    int row = lo * run, req;
+    long long cum = sm.start[lo] * Hkv;
+    int len = dq4_len(p, row, req);
+    while (f < f_end) {
+      while (row + 1 < p.rows && f >= cum + static_cast<long long>(dq4_tiles(len)) * Hkv) {
+        cum += static_cast<long long>(dq4_tiles(len)) * Hkv;
+        len = dq4_len(p, ++row, req);
+      }
+      if (f >= cum + static_cast<long long>(dq4_tiles(len)) * Hkv) break;  // lengths changed under the call
+      const int tiles = dq4_tiles(len);
+      const int kvh = static_cast<int>((f - cum) / tiles);
+      const int t0 = static_cast<int>((f - cum) - static_cast<long long>(kvh) * tiles);
+      const int n = static_cast<int>(min(static_cast<long long>(tiles - t0), f_end - f));
+
+      // ---- Q fragments: columns are heads, lane's k index pairs (d, d + 4)
+      uint32_t qb[NT][2 * KW][2];
+      float sq[NT][NG][2];  // sums of q over each group, heads 2t and 2t+1
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int hc = nt * 8 + g;
+        const uint16_t* qh = static_cast<const uint16_t*>(p.q) + row * p.q_row_stride +
+                             static_cast<long long>(kvh * G + hc) * D;
+        float part[NG];
+#pragma unroll
+        for (int a = 0; a < NG; ++a) part[a] = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          const int grp = w >> 1;
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          if (hc < G) v = *reinterpret_cast<const uint4*>(qh + 64 * grp + 16 * t + 8 * (w & 1));
+          qb[nt][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);      // d, d+4
+          qb[nt][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);      // d+1, d+5
+          qb[nt][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);  // d+2, d+6
+          qb[nt][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);  // d+3, d+7
+          float x[8];
+          q4_unpack8<F16>(v, x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) part[grp] += x[i];
+        }
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          part[a] += __shfl_xor_sync(0xffffffffu, part[a], 1);
+          part[a] += __shfl_xor_sync(0xffffffffu, part[a], 2);
+          sq[nt][a][0] = __shfl_sync(0xffffffffu, part[a], 8 * t);
+          sq[nt][a][1] = __shfl_sync(0xffffffffu, part[a], 8 * t + 4);
+        }
+      }
+      float o[NT][NG][4][4];
+      float vz[NT][NG][2], m_run[NT][2], l_run[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          vz[nt][a][0] = vz[nt][a][1] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[nt][a][i][0] = o[nt][a][i][1] = o[nt][a][i][2] = o[nt][a][i][3] = 0.f;
+        }
+        m_run[nt][0] = m_run[nt][1] = -INFINITY;
+        l_run[nt][0] = l_run[nt][1] = 0.f;
+      }
+
+      // ---- this warp's tiles t0 + warp + 4 i
+      const int cnt = n > warp ? (n - warp + kDq4Warps - 1) / kDq4Warps : 0;
+      const int32_t* bt = p.block_table + req * p.bt_stride;
+      const int sub_mask = (1 << p.sub_shift) - 1;
+      for (int i0 = 0; i0 < cnt; i0 += 32) {
+        int my_blk = -1;
+        if (i0 + lane < cnt) my_blk = bt[(t0 + warp + kDq4Warps * (i0 + lane)) >> p.sub_shift];
+        if (my_blk >= p.num_blocks) my_blk = -1;
+        const int here = min(32, cnt - i0);
+        for (int i = 0; i < here; ++i) {
+          const int blk = __shfl_sync(0xffffffffu, my_blk, i);
+          if (blk < 0) continue;  // a page outside the cache holds no keys
+          const int ti = t0 + warp + kDq4Warps * (i0 + i);
+          const uint8_t* tile = p.cache + (((static_cast<long long>(blk) * Hkv + kvh) << p.sub_shift) + (ti & sub_mask)) *
+                                              L::kTileBytes;
+          Q4Frag<D> fr;
+          q4_load<D>(fr, tile, g, t);
+          const int left = len - 16 * ti;
+          const bool in0 = 2 * g < left, in1 = 2 * g + 1 < left;
+          if (left < 16) {  // keys past the end: unwritten bytes may be anything
+#pragma unroll
+            for (int a = 0; a < 2 * NG; ++a) {
+              fr.prm[0][a] = in0 ? fr.prm[0][a] : 0u;
+              fr.prm[1][a] = in1 ? fr.prm[1][a] : 0u;
+            }
+          }
+          // ---- scores: rows are tokens 2g (c0, c1) and 2g+1 (c2, c3)
+          float sc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+          for (int a = 0; a < NG; ++a) {
+            float acc[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t w0 = fr.k[0][2 * a + e], w1 = fr.k[1][2 * a + e];
+              const uint32_t fa[4] = {q4_pair<F16, 0>(w0), q4_pair<F16, 0>(w1), q4_pair<F16, 1>(w0), q4_pair<F16, 1>(w1)};
+              const uint32_t fb[4] = {q4_pair<F16, 2>(w0), q4_pair<F16, 2>(w1), q4_pair<F16, 3>(w0), q4_pair<F16, 3>(w1)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<F16>(acc[nt], fa, qb[nt][2 * (2 * a + e)][0], qb[nt][2 * (2 * a + e)][1]);
+                mma16816<F16>(acc[nt], fb, qb[nt][2 * (2 * a + e) + 1][0], qb[nt][2 * (2 * a + e) + 1][1]);
+              }
+            }
+            const float s0 = q4_up<F16>(fr.prm[0][a] & 0xffffu), z0 = fmaf(8.f, s0, q4_up<F16>(fr.prm[0][a] >> 16));
+            const float s1 = q4_up<F16>(fr.prm[1][a] & 0xffffu), z1 = fmaf(8.f, s1, q4_up<F16>(fr.prm[1][a] >> 16));
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              sc[nt][0] += fmaf(s0, acc[nt][0], z0 * sq[nt][a][0]);
+              sc[nt][1] += fmaf(s0, acc[nt][1], z0 * sq[nt][a][1]);
+              sc[nt][2] += fmaf(s1, acc[nt][2], z1 * sq[nt][a][0]);
+              sc[nt][3] += fmaf(s1, acc[nt][3], z1 * sq[nt][a][1]);
+            }
+          }
+          bool raise = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[nt][e] = ((e < 2) ? in0 : in1) ? sc[nt][e] * p.scale_log2 : -INFINITY;
+            raise = raise || fmaxf(sc[nt][0], sc[nt][2]) > m_run[nt][0] + kRescaleThreshold ||
+                    fmaxf(sc[nt][1], sc[nt][3]) > m_run[nt][1] + kRescaleThreshold;
+          }
+          if (__any_sync(0xffffffffu, raise)) {
+            // the running base is only raised when a score exceeds it by 8 (p <= 2^8)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                float mx = fmaxf(sc[nt][e], sc[nt][e + 2]);
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+                const float m_new = fmaxf(m_run[nt][e], mx);
+                const float al = m_new == -INFINITY ? 1.f : ex2_approx(m_run[nt][e] - m_new);
+                m_run[nt][e] = m_new;
+                l_run[nt][e] *= al;
+#pragma unroll
+                for (int a = 0; a < NG; ++a) {
+                  vz[nt][a][e] *= al;
+#pragma unroll
+                  for (int i2 = 0; i2 < 4; ++i2) {
+                    o[nt][a][i2][e] *= al;
+                    o[nt][a][i2][e + 2] *= al;
+                  }
+                }
+              }
+          }
+          float pr[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float base = m_run[nt][e & 1] == -INFINITY ? 0.f : m_run[nt][e & 1];
+              pr[nt][e] = ex2_approx(sc[nt][e] - base);
+            }
+            l_run[nt][0] += pr[nt][0] + pr[nt][2];
+            l_run[nt][1] += pr[nt][1] + pr[nt][3];
+          }
+          // ---- O += V^T P per group
+#pragma unroll
+          for (int a = 0; a < NG; ++a) {
+            const float s0 = q4_up<F16>(fr.prm[0][NG + a] & 0xffffu), s1 = q4_up<F16>(fr.prm[1][NG + a] & 0xffffu);
+            const float z0 = fmaf(8.f, s0, q4_up<F16>(fr.prm[0][NG + a] >> 16));
+            const float z1 = fmaf(8.f, s1, q4_up<F16>(fr.prm[1][NG + a] >> 16));
+            uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              vz[nt][a][0] += fmaf(pr[nt][0], z0, pr[nt][2] * z1);
+              vz[nt][a][1] += fmaf(pr[nt][1], z0, pr[nt][3] * z1);
+              const float x0 = pr[nt][0] * s0, x1 = pr[nt][1] * s0, x2 = pr[nt][2] * s1, x3 = pr[nt][3] * s1;
+              const uint32_t h0 = pack2<false>(x0, x1), h1 = pack2<false>(x2, x3);
+              const float2 u0 = unpack2<false>(h0), u1 = unpack2<false>(h1);
+              const uint32_t l0 = pack2<false>(x0 - u0.x, x1 - u0.y), l1 = pack2<false>(x2 - u1.x, x3 - u1.y);
+              bh[nt][0] = movmatrix_t(h0);
+              bh[nt][1] = movmatrix_t(h1);
+              bl[nt][0] = movmatrix_t(l0);
+              bl[nt][1] = movmatrix_t(l1);
+            }
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) {
+              const uint32_t w = fr.v[a][i2];
+              const uint32_t fa[4] = {q4_pair<false, 0>(w), q4_pair<false, 1>(w), q4_pair<false, 2>(w), q4_pair<false, 3>(w)};
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) {
+                mma16816<false>(o[nt][a][i2], fa, bh[nt][0], bh[nt][1]);
+                mma16816<false>(o[nt][a][i2], fa, bl[nt][0], bl[nt][1]);
+              }
+            }
+          }
+        }
+      }
+
+      // ---- join the warps: sums over the lanes' tokens first
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float l = l_run[nt][e];
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+          const int col = nt * 8 + 2 * t + e;
+          if (g == 0) {
+            sm.m[warp][col] = l != l ? 0.f : m_run[nt][e];  // a NaN sum must not hide behind an empty base
+            sm.l[warp][col] = l;
+          }
+#pragma unroll
+          for (int a = 0; a < NG; ++a) {
+            float z = vz[nt][a][e];
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
+#pragma unroll
+            for (int i2 = 0; i2 < 4; ++i2) {
+              float2 v = make_float2(o[nt][a][i2][e] + z, o[nt][a][i2][e + 2] + z);
+              *reinterpret_cast<float2*>(&sm.o[warp][col][8 * (8 * a + g) + 2 * i2]) = v;
+            }
+          }
+        }
+      __syncthreads();
+      const bool whole = n == tiles;
+      const int slot = f == f_begin ? 0 : 1;
+      const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * G;
+      for (int e = tid; e < G * D; e += kDq4Threads) {
+        const int h = e / D, d = e % D;
+        float M = sm.m[0][h];
+#pragma unroll
+        for (int w = 1; w < kDq4Warps; ++w) M = fmaxf(M, sm.m[w][h]);
+        float acc = 0.f, ls = 0.f;
+        if (M != -INFINITY) {
+#pragma unroll
+          for (int w = 0; w < kDq4Warps; ++w) {
+            const float x = ex2_approx(sm.m[w][h] - M);
+            acc = fmaf(x, sm.o[w][h][d], acc);
+            ls = fmaf(x, sm.l[w][h], ls);
+          }
+        }
+        if (whole) {
+          const int head = kvh * G + h;
+          dq4_store(p, row, head, D, d, ls == 0.f ? 0.f : acc / ls);
+          if (d == 0 && p.lse != nullptr)
+            p.lse[head * p.lse_stride + row] = ls == 0.f ? -INFINITY : (M + lg2_approx(ls)) * 0.69314718055994530942f;
+        } else {
+          p.part_o[(part + h) * D + d] = acc;
+          if (d == 0) p.part_ml[part + h] = make_float2(M, ls);
+        }
+      }
+      if (!whole && t0 == 0) {
+        const long long last = (f + tiles - 1) / piece;
+        desc = make_int4(row, kvh, slot, static_cast<int>(last - blockIdx.x) + 1);
+      }
+      __syncthreads();
+      f += n;
+    }
+  }
+  if (tid == 0) p.desc[blockIdx.x] = desc;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Joins the parts of the (row, KV head) whose first part lies in block
+// blockIdx.x, for head blockIdx.y of the group: parts in order, warps by turns.
+template <int D>
+__global__ void __launch_bounds__(128) decode_q4_join_kernel(const __grid_constant__ DecodeQ4Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 desc = p.desc[blockIdx.x];
+  if (desc.x < 0) return;
+  constexpr int V = D / 32;
+  __shared__ float so[4][D], sml[4][2];
+  const int G = p.group, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto index = [&](int i) {
+    return (static_cast<long long>(blockIdx.x + i) * 2 + (i == 0 ? desc.z : 0)) * G + h;
+  };
+  float M = -INFINITY;
+  for (int i = lane; i < desc.w; i += 32) M = fmaxf(M, p.part_ml[index(i)].x);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  float acc[V], ls = 0.f;
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[i] = 0.f;
+  if (M != -INFINITY) {
+#pragma unroll 4
+    for (int i = warp; i < desc.w; i += 4) {
+      const long long at = index(i);
+      const float2 ml = p.part_ml[at];
+      const float x = ex2_approx(ml.x - M);
+      ls = fmaf(x, ml.y, ls);
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(x, p.part_o[at * D + v * 32 + lane], acc[v]);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) so[warp][v * 32 + lane] = acc[v];
+  if (lane == 0) sml[warp][0] = ls;
+  __syncthreads();
+  ls = sml[0][0] + sml[1][0] + sml[2][0] + sml[3][0];
+  const int head = desc.y * G + h;
+  for (int d = threadIdx.x; d < D; d += 128) {
+    const float v = so[0][d] + so[1][d] + so[2][d] + so[3][d];
+    dq4_store(p, desc.x, head, D, d, ls == 0.f ? 0.f : v / ls);
+  }
+  if (threadIdx.x == 0 && p.lse != nullptr)
+    p.lse[head * p.lse_stride + desc.x] = ls == 0.f ? -INFINITY : (M + lg2_approx(ls)) * 0.69314718055994530942f;
+}
+
+}  // namespace hcp

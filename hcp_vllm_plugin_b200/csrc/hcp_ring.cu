@@ -23,6 +23,10 @@
 #include "decode.cuh"
 #include "cache.cuh"
 #include "merge.cuh"
+#include "step_plan.cuh"
+#include "q4_cache.cuh"
+#include "norm_rope.cuh"
+#include "decode_q4.cuh"
 
 namespace hcp {
 namespace {
@@ -52,8 +56,14 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // device is refused (HCP_ERR_INVALID) instead of receiving kernels whose
 // addresses and tensor maps were made for that other device.  0, 1 and 2 are
 // the runtime's default / legacy / per-thread streams of the current device.
+// A stream that is being captured may not be asked for its device (the question
+// ends the capture); there the runtime itself refuses a launch from another device.
 bool stream_on_current_device(void* stream) {
   if (reinterpret_cast<uintptr_t>(stream) <= 2) return true;
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) == cudaSuccess &&
+      capture == cudaStreamCaptureStatusActive)
+    return true;
   int cur = -1, sdev = -1;
   if (cudaGetDevice(&cur) != cudaSuccess) return false;
   if (cudaStreamGetDevice(static_cast<cudaStream_t>(stream), &sdev) != cudaSuccess) {
@@ -862,6 +872,332 @@ extern "C" int hcp_kv_cache_gather(const void* kv_cache, int64_t num_blocks, int
   kv_cache_gather_kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(num_kv_heads)), 256, 0,
                            static_cast<cudaStream_t>(stream)>>>(p);
   return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
+// ---------------------------------------------------------------------------
+// A serving step's data path beside the attention kernels: cache plan, norm and
+// rotation, the 4-bit cache and attention over it.
+// ---------------------------------------------------------------------------
+extern "C" int hcp_kv_plan_step(const hcp_step_plan_args* a, void* stream) {
+  if (!stream_on_current_device(stream)) return HCP_ERR_INVALID;
+  if (a == nullptr || a->num_reqs < 0 || a->num_tokens < 0 || a->block_size <= 0 || a->block_table_width < 0 ||
+      a->block_table_stride < a->block_table_width || a->num_free < 0)
+    return HCP_ERR_INVALID;
+  if (a->free_head == nullptr || a->query_start == nullptr || a->free_head_out == nullptr ||
+      a->free_head_out == a->free_head || a->missing_out == nullptr)
+    return HCP_ERR_INVALID;
+  if (a->num_reqs > 0 && (a->context_lens == nullptr || a->new_lens == nullptr || a->seq_lens == nullptr))
+    return HCP_ERR_INVALID;
+  if (a->num_reqs > 0 && a->block_table_width > 0 && a->block_table == nullptr) return HCP_ERR_INVALID;
+  if (a->num_free > 0 && a->free_blocks == nullptr) return HCP_ERR_INVALID;
+  if (a->num_tokens > 0 && (a->positions == nullptr || a->slot_mapping == nullptr || a->token_req == nullptr ||
+                            a->kv_lens == nullptr))
+    return HCP_ERR_INVALID;
+  if (a->num_tokens > INT32_MAX || a->block_table_width > INT32_MAX || a->num_free > INT32_MAX)
+    return HCP_ERR_UNSUPPORTED;
+  StepPlanParams p;
+  p.context_lens = a->context_lens;
+  p.new_lens = a->new_lens;
+  p.pos_base = a->pos_base;
+  p.block_table = a->block_table;
+  p.bt_stride = a->block_table_stride;
+  p.bt_width = a->block_table_width;
+  p.free_blocks = a->free_blocks;
+  p.num_free = a->num_free;
+  p.free_head = a->free_head;
+  p.query_start = a->query_start;
+  p.seq_lens = a->seq_lens;
+  p.positions = a->positions;
+  p.slot_mapping = a->slot_mapping;
+  p.token_req = a->token_req;
+  p.kv_lens = a->kv_lens;
+  p.free_head_out = a->free_head_out;
+  p.missing = a->missing_out;
+  p.num_reqs = a->num_reqs;
+  p.num_tokens = a->num_tokens;
+  p.block_size = a->block_size;
+  const int64_t blocks = std::max<int64_t>(1, (a->num_tokens + kPlanThreads - 1) / kPlanThreads);
+  step_plan_kernel<<<static_cast<int>(std::min<int64_t>(blocks, 2 * 148)), kPlanThreads, 0,
+                     static_cast<cudaStream_t>(stream)>>>(p);
+  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
+namespace {
+
+bool q4_block_size(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128; }
+bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
+
+template <int D, bool F16, bool TAB32>
+int launch_norm_rope(const NormRopeParams& p, int64_t tokens, int kind, cudaStream_t st) {
+  constexpr int per_round = kRopeThreads / (D / 8);
+  const int rows = p.num_heads + p.num_kv_heads * (kind == HCP_ROPE_CACHE_NONE ? 1 : 2);
+  const int rounds = (rows + per_round - 1) / per_round;
+  // few tokens: one round a block, so the whole token is in flight at once
+  const int spread = tokens * rounds <= 8 * 148 ? rounds : 1;
+  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(spread));
+  switch (kind) {
+    case HCP_ROPE_CACHE_SAME: norm_rope_kernel<D, F16, TAB32, kRopeCacheSame><<<grid, kRopeThreads, 0, st>>>(p); break;
+    case HCP_ROPE_CACHE_Q4: norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4><<<grid, kRopeThreads, 0, st>>>(p); break;
+    default: norm_rope_kernel<D, F16, TAB32, kRopeCacheNone><<<grid, kRopeThreads, 0, st>>>(p); break;
+  }
+  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
+template <int D, bool F16, int NT>
+int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
+  decode_q4_kernel<D, F16, NT><<<kDq4Ctas, kDq4Threads, 0, st>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return HCP_ERR_CUDA;
+  // the joining kernel may start while the first one ends; it waits for it itself
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(kDq4Ctas, static_cast<unsigned>(p.group));
+  cfg.blockDim = dim3(128);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D>, p) == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
+int validate_decode_q4(const hcp_decode_q4_args* a) {
+  if (a == nullptr) return HCP_ERR_INVALID;
+  if (a->dtype != HCP_BF16 && a->dtype != HCP_F16) return HCP_ERR_UNSUPPORTED;
+  const int H = a->num_heads, Hkv = a->num_kv_heads, D = a->head_dim;
+  if (H <= 0 || Hkv <= 0 || H % Hkv != 0) return HCP_ERR_INVALID;
+  if (H / Hkv > kDecMaxGroup || (D != 64 && D != 128) || !q4_block_size(a->block_size)) return HCP_ERR_UNSUPPORTED;
+  if (a->out_dtype != a->dtype && a->out_dtype != HCP_F32) return HCP_ERR_UNSUPPORTED;
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return HCP_ERR_INVALID;
+  if (a->q_rows < 0) return HCP_ERR_INVALID;
+  if (a->q_rows > INT32_MAX / 2) return HCP_ERR_UNSUPPORTED;
+  if (a->q_rows == 0) return HCP_OK;
+  const int64_t row = static_cast<int64_t>(H) * D;
+  if (a->q == nullptr || a->out == nullptr || a->kv_lens == nullptr || a->q_row_stride < row || a->out_row_stride < row ||
+      (a->q_row_stride % 8) != 0 || !aligned16(a->q))
+    return HCP_ERR_INVALID;
+  if (a->kv_cache == nullptr || a->num_blocks <= 0 || a->num_blocks >= (1ll << 31) || !aligned16(a->kv_cache) ||
+      a->block_table == nullptr || a->block_table_rows <= 0 || a->block_table_width <= 0 ||
+      a->block_table_stride < a->block_table_width)
+    return HCP_ERR_INVALID;
+  if (a->block_table_width > INT32_MAX / a->block_size - 1) return HCP_ERR_UNSUPPORTED;
+  if (a->token_req == nullptr && a->block_table_rows < a->q_rows) return HCP_ERR_INVALID;
+  if (a->lse != nullptr && a->lse_stride < a->q_rows) return HCP_ERR_INVALID;
+  return HCP_OK;
+}
+
+// Workspace: descriptors, then (base, sum) pairs, then partial sums, each 16-byte aligned.
+int64_t dq4_desc_bytes() { return static_cast<int64_t>(kDq4Ctas) * 16; }
+int64_t dq4_ml_bytes(int group) { return static_cast<int64_t>(kDq4Ctas) * 2 * group * 8; }
+
+}  // namespace
+
+extern "C" int hcp_qk_norm_rope(const hcp_norm_rope_args* a, void* stream) {
+  if (!stream_on_current_device(stream)) return HCP_ERR_INVALID;
+  if (a == nullptr) return HCP_ERR_INVALID;
+  if (a->dtype != HCP_BF16 && a->dtype != HCP_F16) return HCP_ERR_UNSUPPORTED;
+  const int H = a->num_heads, Hkv = a->num_kv_heads, D = a->head_dim;
+  if (H <= 0 || Hkv <= 0) return HCP_ERR_INVALID;
+  if ((D != 64 && D != 128) || H > 4096 || Hkv > 4096) return HCP_ERR_UNSUPPORTED;
+  if (a->table_dtype != HCP_F32 && a->table_dtype != a->dtype) return HCP_ERR_UNSUPPORTED;
+  if (a->rotary <= 0 || a->rotary > D || a->rotary % 8 != 0) return HCP_ERR_UNSUPPORTED;
+  if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return HCP_ERR_INVALID;
+  if (a->num_tokens < 0 || a->table_rows < 0) return HCP_ERR_INVALID;
+  if (a->cache_kind != HCP_ROPE_CACHE_NONE && a->cache_kind != HCP_ROPE_CACHE_SAME && a->cache_kind != HCP_ROPE_CACHE_Q4)
+    return HCP_ERR_INVALID;
+  const bool cached = a->cache_kind != HCP_ROPE_CACHE_NONE;
+  if (cached && (a->block_size <= 0 || a->num_blocks <= 0)) return HCP_ERR_INVALID;
+  if (a->cache_kind == HCP_ROPE_CACHE_Q4 && !q4_block_size(a->block_size)) return HCP_ERR_UNSUPPORTED;
+  if (a->num_tokens > INT32_MAX) return HCP_ERR_UNSUPPORTED;
+  if (a->num_tokens == 0) return HCP_OK;
+  const int64_t q_row = static_cast<int64_t>(H) * D, kv_row = static_cast<int64_t>(Hkv) * D;
+  auto rows_ok = [](const void* base, int64_t stride, int64_t row) {
+    return base != nullptr && aligned16(base) && stride >= row && stride % 8 == 0;
+  };
+  if (!rows_ok(a->q, a->q_row_stride, q_row) || !rows_ok(a->q_out, a->q_out_row_stride, q_row) ||
+      !rows_ok(a->k, a->k_row_stride, kv_row) || !rows_ok(a->k_out, a->k_out_row_stride, kv_row))
+    return HCP_ERR_INVALID;
+  if (cached && (!rows_ok(a->v, a->v_row_stride, kv_row) || a->kv_cache == nullptr || !aligned16(a->kv_cache) ||
+                 a->slot_mapping == nullptr))
+    return HCP_ERR_INVALID;
+  if (a->positions == nullptr || a->cos_sin == nullptr || !aligned16(a->cos_sin) || a->table_stride < a->rotary ||
+      a->table_stride % 4 != 0)
+    return HCP_ERR_INVALID;
+  if ((a->q_weight != nullptr && !aligned8(a->q_weight)) || (a->k_weight != nullptr && !aligned8(a->k_weight)))
+    return HCP_ERR_INVALID;
+  NormRopeParams p;
+  p.q = static_cast<const uint16_t*>(a->q);
+  p.k = static_cast<const uint16_t*>(a->k);
+  p.v = static_cast<const uint16_t*>(a->v);
+  p.q_out = static_cast<uint16_t*>(a->q_out);
+  p.k_out = static_cast<uint16_t*>(a->k_out);
+  p.q_stride = a->q_row_stride;
+  p.k_stride = a->k_row_stride;
+  p.v_stride = a->v_row_stride;
+  p.q_out_stride = a->q_out_row_stride;
+  p.k_out_stride = a->k_out_row_stride;
+  p.positions = a->positions;
+  p.table = a->cos_sin;
+  p.table_stride = a->table_stride;
+  p.table_rows = a->table_rows;
+  p.q_weight = static_cast<const uint16_t*>(a->q_weight);
+  p.k_weight = static_cast<const uint16_t*>(a->k_weight);
+  p.slot_mapping = a->slot_mapping;
+  p.cache = a->kv_cache;
+  p.num_blocks = a->num_blocks;
+  p.eps = a->eps;
+  p.num_heads = H;
+  p.num_kv_heads = Hkv;
+  p.rotary = a->rotary;
+  p.interleaved = a->interleaved;
+  p.block_size = a->block_size;
+  p.bs_shift = pow2_shift(a->block_size);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->dtype == HCP_F16, tab32 = a->table_dtype == HCP_F32;
+  const int64_t n = a->num_tokens;
+  const int kind = a->cache_kind;
+  if (D == 128) {
+    if (f16) return tab32 ? launch_norm_rope<128, true, true>(p, n, kind, st) : launch_norm_rope<128, true, false>(p, n, kind, st);
+    return tab32 ? launch_norm_rope<128, false, true>(p, n, kind, st) : launch_norm_rope<128, false, false>(p, n, kind, st);
+  }
+  if (f16) return tab32 ? launch_norm_rope<64, true, true>(p, n, kind, st) : launch_norm_rope<64, true, false>(p, n, kind, st);
+  return tab32 ? launch_norm_rope<64, false, true>(p, n, kind, st) : launch_norm_rope<64, false, false>(p, n, kind, st);
+}
+
+namespace {
+// Shared checks of the 4-bit scatter and gather; HCP_OK with num_tokens 0 means nothing to do.
+int validate_q4_rows(const void* key, const void* value, int64_t num_tokens, int64_t key_row_stride,
+                     int64_t value_row_stride, const int64_t* slot_mapping, const void* kv_cache, int64_t num_blocks,
+                     int32_t block_size, int32_t num_kv_heads, int32_t head_dim, int32_t dtype) {
+  if (dtype != HCP_BF16 && dtype != HCP_F16) return HCP_ERR_UNSUPPORTED;
+  if (num_tokens < 0 || num_kv_heads <= 0 || num_blocks <= 0) return HCP_ERR_INVALID;
+  if ((head_dim != 64 && head_dim != 128) || !q4_block_size(block_size) || num_kv_heads > 65535)
+    return HCP_ERR_UNSUPPORTED;
+  if (num_tokens > INT32_MAX) return HCP_ERR_UNSUPPORTED;
+  if (num_tokens == 0) return HCP_OK;
+  const int64_t row = static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (key == nullptr || value == nullptr || slot_mapping == nullptr || kv_cache == nullptr || key_row_stride < row ||
+      value_row_stride < row || (key_row_stride % 8) != 0 || (value_row_stride % 8) != 0 || !aligned16(key) ||
+      !aligned16(value) || !aligned16(kv_cache))
+    return HCP_ERR_INVALID;
+  return HCP_OK;
+}
+}  // namespace
+
+extern "C" int hcp_kv_cache_update_q4(const void* key, const void* value, int64_t num_tokens, int64_t key_row_stride,
+                                      int64_t value_row_stride, const int64_t* slot_mapping, void* kv_cache,
+                                      int64_t num_blocks, int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                                      int32_t dtype, void* stream) {
+  if (!stream_on_current_device(stream)) return HCP_ERR_INVALID;
+  const int rc = validate_q4_rows(key, value, num_tokens, key_row_stride, value_row_stride, slot_mapping, kv_cache,
+                                  num_blocks, block_size, num_kv_heads, head_dim, dtype);
+  if (rc != HCP_OK || num_tokens == 0) return rc;
+  Q4UpdateParams p;
+  p.key = static_cast<const uint16_t*>(key);
+  p.value = static_cast<const uint16_t*>(value);
+  p.key_row_stride = key_row_stride;
+  p.value_row_stride = value_row_stride;
+  p.slot_mapping = slot_mapping;
+  p.cache = static_cast<uint8_t*>(kv_cache);
+  p.num_blocks = num_blocks;
+  p.num_tokens = num_tokens;
+  p.block_size = block_size;
+  p.bs_shift = pow2_shift(block_size);
+  p.num_kv_heads = num_kv_heads;
+  const int per_block = 256 / (head_dim / 4);
+  const dim3 grid(static_cast<unsigned>((num_tokens + per_block - 1) / per_block), static_cast<unsigned>(num_kv_heads));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128) {
+    if (dtype == HCP_F16) q4_update_kernel<128, true><<<grid, 256, 0, st>>>(p);
+    else q4_update_kernel<128, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (dtype == HCP_F16) q4_update_kernel<64, true><<<grid, 256, 0, st>>>(p);
+    else q4_update_kernel<64, false><<<grid, 256, 0, st>>>(p);
+  }
+  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
+extern "C" int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, int32_t block_size,
+                                      int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping,
+                                      int64_t num_tokens, void* key, void* value, int64_t key_row_stride,
+                                      int64_t value_row_stride, int32_t dtype, void* stream) {
+  if (!stream_on_current_device(stream)) return HCP_ERR_INVALID;
+  const int rc = validate_q4_rows(key, value, num_tokens, key_row_stride, value_row_stride, slot_mapping, kv_cache,
+                                  num_blocks, block_size, num_kv_heads, head_dim, dtype);
+  if (rc != HCP_OK || num_tokens == 0) return rc;
+  Q4GatherParams p;
+  p.cache = static_cast<const uint8_t*>(kv_cache);
+  p.slot_mapping = slot_mapping;
+  p.key = static_cast<uint16_t*>(key);
+  p.value = static_cast<uint16_t*>(value);
+  p.key_row_stride = key_row_stride;
+  p.value_row_stride = value_row_stride;
+  p.num_blocks = num_blocks;
+  p.num_tokens = num_tokens;
+  p.block_size = block_size;
+  p.bs_shift = pow2_shift(block_size);
+  p.num_kv_heads = num_kv_heads;
+  const int per_block = 256 / (head_dim / 4);
+  const dim3 grid(static_cast<unsigned>((num_tokens + per_block - 1) / per_block), static_cast<unsigned>(num_kv_heads));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (head_dim == 128) {
+    if (dtype == HCP_F16) q4_gather_kernel<128, true><<<grid, 256, 0, st>>>(p);
+    else q4_gather_kernel<128, false><<<grid, 256, 0, st>>>(p);
+  } else {
+    if (dtype == HCP_F16) q4_gather_kernel<64, true><<<grid, 256, 0, st>>>(p);
+    else q4_gather_kernel<64, false><<<grid, 256, 0, st>>>(p);
+  }
+  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
+extern "C" int64_t hcp_decode_q4_workspace_bytes(const hcp_decode_q4_args* a) {
+  if (validate_decode_q4(a) != HCP_OK) return -1;
+  const int G = a->num_heads / a->num_kv_heads;
+  return dq4_desc_bytes() + dq4_ml_bytes(G) + static_cast<int64_t>(kDq4Ctas) * 2 * G * a->head_dim * 4;
+}
+
+extern "C" int hcp_decode_q4_splitkv(const hcp_decode_q4_args* a, void* stream) {
+  if (!stream_on_current_device(stream)) return HCP_ERR_INVALID;
+  const int rc = validate_decode_q4(a);
+  if (rc != HCP_OK) return rc;
+  if (a->q_rows == 0) return HCP_OK;
+  if (a->workspace == nullptr || !aligned16(a->workspace) || a->workspace_bytes < hcp_decode_q4_workspace_bytes(a))
+    return HCP_ERR_INVALID;
+  const int G = a->num_heads / a->num_kv_heads;
+  DecodeQ4Params p;
+  p.q = a->q;
+  p.q_row_stride = a->q_row_stride;
+  p.cache = static_cast<const uint8_t*>(a->kv_cache);
+  p.block_table = a->block_table;
+  p.bt_stride = a->block_table_stride;
+  p.bt_width = a->block_table_width;
+  p.bt_rows = a->block_table_rows;
+  p.num_blocks = a->num_blocks;
+  p.kv_lens = a->kv_lens;
+  p.token_req = a->token_req;
+  p.out = a->out;
+  p.out_row_stride = a->out_row_stride;
+  p.lse = a->lse;
+  p.lse_stride = a->lse_stride;
+  char* ws = static_cast<char*>(a->workspace);
+  p.desc = reinterpret_cast<int4*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + dq4_desc_bytes());
+  p.part_o = reinterpret_cast<float*>(ws + dq4_desc_bytes() + dq4_ml_bytes(G));
+  p.rows = static_cast<int>(a->q_rows);
+  p.num_heads = a->num_heads;
+  p.num_kv_heads = a->num_kv_heads;
+  p.group = G;
+  p.block_size = a->block_size;
+  p.sub_shift = pow2_shift(a->block_size / kQ4TileTokens);
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.out_dt = a->out_dtype;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool f16 = a->dtype == HCP_F16, wide = G > 8;
+  if (a->head_dim == 128) {
+    if (f16) return wide ? launch_decode_q4<128, true, 2>(p, st) : launch_decode_q4<128, true, 1>(p, st);
+    return wide ? launch_decode_q4<128, false, 2>(p, st) : launch_decode_q4<128, false, 1>(p, st);
+  }
+  if (f16) return wide ? launch_decode_q4<64, true, 2>(p, st) : launch_decode_q4<64, true, 1>(p, st);
+  return wide ? launch_decode_q4<64, false, 2>(p, st) : launch_decode_q4<64, false, 1>(p, st);
 }
 
 // ---------------------------------------------------------------------------

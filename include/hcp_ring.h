@@ -270,6 +270,148 @@ int hcp_kv_cache_gather(const void* kv_cache, int64_t num_blocks, int32_t block_
                         int64_t num_tokens, void* key, void* value, int64_t key_row_stride,
                         int64_t value_row_stride, int32_t dtype, void* stream);
 
+/*
+ * One engine step's cache plan from the requests' lengths, on the GPU: the new
+ * blocks of every request go into its block_table row and every new token gets
+ * its request, position, cache slot and number of visible keys.  One launch, no
+ * host read; with padded buffers it can be captured.
+ *
+ *   request i holds context_lens[i] tokens and gets new_lens[i] (negative = 0);
+ *   it needs ceil((context + new) / block_size) blocks, at most
+ *   block_table_width, and has ceil(context / block_size); the rest are taken in
+ *   request order from free_blocks[*free_head ...] (-1 where the list ends);
+ *   token t of the step (requests in order): position pos_base[i] + p, p counted
+ *   in the request, slot block * block_size + p % block_size (-1 without a
+ *   block), kv_len p + 1.
+ * Rows past the step's last token: position, slot and request -1, kv_len 0.
+ * Only the new entries of block_table are written, so a call can be repeated.
+ * *missing_out: blocks that were needed and not given (list or row exhausted).
+ *
+ * Replaces: the host-side block and slot bookkeeping a serving engine does per
+ * step before it calls do_kv_cache_update (hcp_vllm_plugin/ring_backend.py:
+ * 501-539 reads attn_metadata's slot_mapping).
+ */
+typedef struct hcp_step_plan_args {
+  const int32_t* context_lens;   /* [num_reqs] */
+  const int32_t* new_lens;       /* [num_reqs] */
+  const int32_t* pos_base;       /* [num_reqs] or NULL (0): global position of the
+                                    request's first cached token */
+  int32_t* block_table;          int64_t block_table_stride; int64_t block_table_width;
+  const int32_t* free_blocks;    int64_t num_free;
+  const int32_t* free_head;      /* [1] entries of free_blocks already taken */
+  int32_t* query_start;          /* [num_reqs + 1] */
+  int32_t* seq_lens;             /* [num_reqs] context + new */
+  int64_t* positions;            /* [num_tokens] */
+  int64_t* slot_mapping;         /* [num_tokens] */
+  int32_t* token_req;            /* [num_tokens] */
+  int32_t* kv_lens;              /* [num_tokens] */
+  int32_t* free_head_out;        /* [1], may not alias free_head */
+  int32_t* missing_out;          /* [1] */
+  int32_t num_reqs;
+  int32_t block_size;
+  int64_t num_tokens;
+} hcp_step_plan_args;
+int hcp_kv_plan_step(const hcp_step_plan_args* args, void* stream);
+
+/*
+ * Per-head RMS norm and position rotation of queries and keys in one pass, and
+ * with a cache the write of keys and values into it:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight    (weight NULL: y = x)
+ *   pairs (a, b) -> (a cos - b sin, b cos + a sin), pair i of rotary / 2 being
+ *   dims (i, i + rotary / 2), or (2i, 2i + 1) with interleaved != 0; dims past
+ *   `rotary` keep y.  cos_sin [table_rows, rotary]: cos, then sin.
+ * 32-bit arithmetic, one rounding to dtype; the cache holds the rounded keys.
+ * q_out / k_out may be q / k themselves.  A negative position marks a padding
+ * row: its outputs and slot stay as they were.  A position past the table gives
+ * NaN rows and leaves its slot.  Slots as in hcp_kv_cache_update.
+ */
+typedef enum hcp_rope_cache {
+  HCP_ROPE_CACHE_NONE = 0,
+  HCP_ROPE_CACHE_SAME = 1,  /* [num_blocks, Hkv, block_size, 2*D] of dtype */
+  HCP_ROPE_CACHE_Q4 = 2     /* the 4-bit cache below */
+} hcp_rope_cache;
+typedef struct hcp_norm_rope_args {
+  int32_t dtype;                 /* HCP_BF16 or HCP_F16 */
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;              /* 64 or 128 */
+  const void* q;                 int64_t q_row_stride;
+  const void* k;                 int64_t k_row_stride;
+  const void* v;                 int64_t v_row_stride;      /* with a cache */
+  void* q_out;                   int64_t q_out_row_stride;
+  void* k_out;                   int64_t k_out_row_stride;
+  const int64_t* positions;      int64_t num_tokens;
+  const void* cos_sin;           int64_t table_rows; int64_t table_stride;
+  int32_t table_dtype;           /* HCP_F32 or dtype */
+  int32_t rotary;                /* multiple of 8, <= head_dim */
+  int32_t interleaved;
+  float eps;
+  const void* q_weight;          const void* k_weight;      /* [D] of dtype, or NULL */
+  void* kv_cache;                const int64_t* slot_mapping;
+  int64_t num_blocks;
+  int32_t block_size;
+  int32_t cache_kind;            /* hcp_rope_cache */
+} hcp_norm_rope_args;
+int hcp_qk_norm_rope(const hcp_norm_rope_args* args, void* stream);
+
+/*
+ * The 4-bit paged cache: uint8 [num_blocks, Hkv, block_size, 9*D/8], block_size
+ * 16, 32, 64 or 128, D 64 or 128.  Every 64 dims of a token, head and side (K, V)
+ * hold a scale s and lowest value m in the rows' 16-bit dtype and whole numbers
+ * n in 0..15:
+ *   s = round16((max - min) / 15), m = min, n = round((x - m) / s), x' = m + s n
+ * (ties to even; s = 0: n = 0).  A group with an infinity or NaN, or whose range
+ * overflows 32 bits, reads back as NaN.  The bytes' order is the library's own
+ * (q4_cache.cuh); the dtype of the calls that read must be the one that wrote.
+ *
+ * hcp_kv_cache_update_q4 / hcp_kv_cache_gather_q4: as hcp_kv_cache_update /
+ * hcp_kv_cache_gather, on it.  A slot named twice in one update holds a mixture
+ * of its rows.
+ */
+int hcp_kv_cache_update_q4(const void* key, const void* value, int64_t num_tokens,
+                           int64_t key_row_stride, int64_t value_row_stride,
+                           const int64_t* slot_mapping, void* kv_cache, int64_t num_blocks,
+                           int32_t block_size, int32_t num_kv_heads, int32_t head_dim,
+                           int32_t dtype, void* stream);
+int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, int32_t block_size,
+                           int32_t num_kv_heads, int32_t head_dim, const int64_t* slot_mapping,
+                           int64_t num_tokens, void* key, void* value, int64_t key_row_stride,
+                           int64_t value_row_stride, int32_t dtype, void* stream);
+
+/*
+ * Attention of single query rows over the 4-bit paged cache.  Row r attends the
+ * first kv_lens[r] keys of block_table row token_req[r] (NULL: row r), all
+ * visible; several rows may name one request (a causal chunk: kv_lens = position
+ * + 1).  Lengths, requests and pages are read on the GPU.
+ *   kv_lens[r] <= 0: out 0, lse -inf.  A request outside the table (negative, say)
+ *   marks a padding row: out and lse stay as they were.  Lengths are cut to
+ *   block_table_width * block_size; a page outside the cache holds no keys.
+ * Needs hcp_decode_q4_workspace_bytes(args) bytes of 16-byte aligned device
+ * workspace (its contents need no preparation; calls that may overlap on the GPU
+ * need their own).
+ */
+typedef struct hcp_decode_q4_args {
+  int32_t dtype;                 /* HCP_BF16 or HCP_F16 */
+  int32_t num_heads;
+  int32_t num_kv_heads;          /* num_heads / num_kv_heads <= 16 */
+  int32_t head_dim;              /* 64 or 128 */
+  float scale;
+  int32_t block_size;            /* 16, 32, 64 or 128 */
+  const void* q;                 int64_t q_rows; int64_t q_row_stride;
+  const void* kv_cache;          int64_t num_blocks;
+  const int32_t* block_table;    int64_t block_table_rows; int64_t block_table_stride;
+  int64_t block_table_width;
+  const int32_t* kv_lens;        /* [q_rows] */
+  const int32_t* token_req;      /* [q_rows] or NULL */
+  void* out;                     int64_t out_row_stride;
+  int32_t out_dtype;             /* dtype or HCP_F32 */
+  int32_t _pad0;
+  float* lse;                    int64_t lse_stride;       /* [H, lse_stride], may be NULL */
+  void* workspace;               int64_t workspace_bytes;
+} hcp_decode_q4_args;
+int hcp_decode_q4_splitkv(const hcp_decode_q4_args* args, void* stream);
+int64_t hcp_decode_q4_workspace_bytes(const hcp_decode_q4_args* args);
+
 /* Bytes of the fixed device array behind hcp_ring_decode_splitkv_noalloc. */
 #define HCP_DECODE_NOALLOC_SCRATCH_BYTES (16LL * 1024 * 1024)
 
