@@ -40,10 +40,11 @@ namespace hcp {
 
 constexpr int kDq4Warps = 4;
 constexpr int kDq4Threads = kDq4Warps * 32;
-constexpr int kDq4CtasPerSm = 3;
+constexpr int kDq4CtasPerSm = 4;
 constexpr int kDq4Sms = 148;
 constexpr int kDq4Ctas = kDq4Sms * kDq4CtasPerSm;
 constexpr int kDq4MinTiles = kDq4Warps;  // tiles of a piece at least: one a warp
+constexpr int kDq4Stages = 4;            // tiles of a warp's ring: one read, the others in flight
 
 struct DecodeQ4Params {
   const void* q;
@@ -73,17 +74,13 @@ struct DecodeQ4Params {
   int out_dt;
 };
 
-__device__ __forceinline__ uint4 ldg_stream(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
+__device__ __forceinline__ void cp_async16(uint32_t dst, const uint8_t* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ uint2 ldg_stream2(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   uint32_t d;
@@ -91,53 +88,20 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   return d;
 }
 
-// Nibbles I and I+4 of a word as a pair n - 8 in 16 bits: with the nibble in the
-// low mantissa bits of 128 (bf16) or 1024 (fp16) the value is 128 + n or 1024 + n,
-// and the subtraction is exact.
+// Nibbles I and I+4 of a word as a pair 16 + n in 16 bits: the nibble becomes the
+// upper mantissa bits of 16.
 template <bool F16, int I>
-__device__ __forceinline__ uint32_t q4_pair(uint32_t w) {
-  constexpr uint32_t kBase = F16 ? 0x64006400u : 0x43004300u;
-  const uint32_t v = ((w >> (4 * I)) & 0x000f000fu) | kBase;
-  if constexpr (F16) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __floats2half2_rn(1032.f, 1032.f));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(136.f, 136.f));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
+__device__ __forceinline__ uint32_t q4_pair16(uint32_t w) {
+  constexpr int kAt = F16 ? 6 : 3;  // lowest mantissa bit that counts 1
+  const uint32_t v = 4 * I > kAt ? w >> (4 * I > kAt ? 4 * I - kAt : 0) : w << (4 * I > kAt ? 0 : kAt - 4 * I);
+  return F16 ? (v & 0x03c003c0u) | 0x4c004c00u : (v & 0x00780078u) | 0x41804180u;
 }
-
-// A lane's share of one tile: K rows of tokens 2g and 2g+1, V pieces, parameters
-// of both tokens.
-template <int D>
-struct Q4Frag {
-  uint32_t k[2][4 * Q4<D>::kGroups / 2];  // D = 128: 4 words a token; 64: 2
-  uint32_t v[Q4<D>::kGroups][4];
-  uint32_t prm[2][2 * Q4<D>::kGroups];    // per token: K (s, lo) of each group, then V
-};
-
-template <int D>
-__device__ __forceinline__ void q4_load(Q4Frag<D>& f, const uint8_t* tile, int g, int t) {
-  using L = Q4<D>;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const uint8_t* kp = tile + (2 * g + e) * (D / 2) + t * (D / 8);
-    const uint8_t* pp = tile + L::kParamOff + (2 * g + e) * L::kTokenParams;
-    if constexpr (D == 128) {
-      const uint4 a = ldg_stream(kp), b = ldg_stream(pp);
-      f.k[e][0] = a.x; f.k[e][1] = a.y; f.k[e][2] = a.z; f.k[e][3] = a.w;
-      f.prm[e][0] = b.x; f.prm[e][1] = b.y; f.prm[e][2] = b.z; f.prm[e][3] = b.w;
-    } else {
-      const uint2 a = ldg_stream2(kp), b = ldg_stream2(pp);
-      f.k[e][0] = a.x; f.k[e][1] = a.y;
-      f.prm[e][0] = b.x; f.prm[e][1] = b.y;
-    }
-  }
-#pragma unroll
-  for (int hf = 0; hf < L::kGroups; ++hf) {
-    const uint4 a = ldg_stream(tile + L::kVOff + (hf * 8 + g) * 64 + t * 16);
-    f.v[hf][0] = a.x; f.v[hf][1] = a.y; f.v[hf][2] = a.z; f.v[hf][3] = a.w;
-  }
+// ... and as a pair n - 8 in bf16: 128 + n from the lowest mantissa bits, minus 136 (exact).
+template <int I>
+__device__ __forceinline__ uint32_t q4_pair_centred(uint32_t w) {
+  const uint32_t v = ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
+  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(136.f, 136.f));
+  return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // Tiles of a row (0 for a padding row or an empty one).
@@ -153,7 +117,12 @@ template <int D, int NT>
 struct Dq4Smem {
   static constexpr int kCols = 8 * NT;
   static constexpr int kPitch = D + 4;
-  float o[kDq4Warps][kCols][kPitch];
+  // the warps' rings of tiles; once a piece of a row is through, its sums
+  static constexpr int kRing = kDq4Stages * Q4<D>::kTileBytes;
+  union {
+    alignas(16) uint8_t ring[kDq4Warps][kRing];
+    float o[kDq4Warps][kCols][kPitch];
+  };
   float m[kDq4Warps][kCols];
   float l[kDq4Warps][kCols];
   long long start[kDq4Threads + 1];
@@ -177,6 +146,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, t = lane & 3;
   const int G = p.group, Hkv = p.num_kv_heads;
+  const uint32_t ring = ptx::smem_u32(sm.ring[warp]);
 
   // ---- the line of tiles: sums of every thread's run of rows
   const int run = (p.rows + kDq4Threads - 1) / kDq4Threads;
@@ -268,7 +238,8 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
         }
       }
       float o[NT][NG][4][4];
-      float vz[NT][NG][2], m_run[NT][2], l_run[NT][2];
+      float vz[NT][NG][2], l_run[NT][2];
+      float limit[NT][2];  // base of the weights + 8; the base is the running maximum or up to 8 below it
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -277,143 +248,199 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][a][i][0] = o[nt][a][i][1] = o[nt][a][i][2] = o[nt][a][i][3] = 0.f;
         }
-        m_run[nt][0] = m_run[nt][1] = -INFINITY;
+        limit[nt][0] = limit[nt][1] = -INFINITY;
         l_run[nt][0] = l_run[nt][1] = 0.f;
       }
 
-      // ---- this warp's tiles t0 + warp + 4 i
+      // ---- this warp's tiles t0 + warp + 4 i, i < cnt, through its ring
       const int cnt = n > warp ? (n - warp + kDq4Warps - 1) / kDq4Warps : 0;
       const int32_t* bt = p.block_table + req * p.bt_stride;
       const int sub_mask = (1 << p.sub_shift) - 1;
-      for (int i0 = 0; i0 < cnt; i0 += 32) {
-        int my_blk = -1;
-        if (i0 + lane < cnt) my_blk = bt[(t0 + warp + kDq4Warps * (i0 + lane)) >> p.sub_shift];
-        if (my_blk >= p.num_blocks) my_blk = -1;
-        const int here = min(32, cnt - i0);
-        for (int i = 0; i < here; ++i) {
-          const int blk = __shfl_sync(0xffffffffu, my_blk, i);
-          if (blk < 0) continue;  // a page outside the cache holds no keys
-          const int ti = t0 + warp + kDq4Warps * (i0 + i);
-          const uint8_t* tile = p.cache + (((static_cast<long long>(blk) * Hkv + kvh) << p.sub_shift) + (ti & sub_mask)) *
-                                              L::kTileBytes;
-          Q4Frag<D> fr;
-          q4_load<D>(fr, tile, g, t);
-          const int left = len - 16 * ti;
-          const bool in0 = 2 * g < left, in1 = 2 * g + 1 < left;
-          if (left < 16) {  // keys past the end: unwritten bytes may be anything
-#pragma unroll
-            for (int a = 0; a < 2 * NG; ++a) {
-              fr.prm[0][a] = in0 ? fr.prm[0][a] : 0u;
-              fr.prm[1][a] = in1 ? fr.prm[1][a] : 0u;
-            }
+      const int first = t0 + warp;
+      // page of tile 32 b + lane; the next 32 are on their way while these are used
+      auto pages = [&](int b) {
+        int v = -1;
+        if (32 * b + lane < cnt) v = __ldg(bt + ((first + kDq4Warps * (32 * b + lane)) >> p.sub_shift));
+        return v < p.num_blocks ? v : -1;
+      };
+      int page = pages(0), page_next = pages(1);
+      uint32_t held = 0;  // bit k: the tile issued k before the last one has a page
+      auto issue = [&](int i) {
+        int blk = -1;
+        if (i < cnt) {
+          if (i > 0 && (i & 31) == 0) {
+            page = page_next;
+            page_next = pages((i >> 5) + 1);
           }
-          // ---- scores: rows are tokens 2g (c0, c1) and 2g+1 (c2, c3)
-          float sc[NT][4];
+          blk = __shfl_sync(0xffffffffu, page, i & 31);
+          if (blk >= 0) {
+            const int ti = first + kDq4Warps * i;
+            const uint8_t* src = p.cache + (((static_cast<long long>(blk) * Hkv + kvh) << p.sub_shift) + (ti & sub_mask)) *
+                                               L::kTileBytes + 16 * lane;
+            const uint32_t dst = ring + (i % kDq4Stages) * L::kTileBytes + 16 * lane;
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+            for (int c = 0; c < L::kTileBytes / 512; ++c) cp_async16(dst + 512 * c, src + 512 * c);
+            constexpr int kRest = L::kTileBytes % 512 / 16;
+            if (lane < kRest) cp_async16(dst + L::kTileBytes / 512 * 512, src + L::kTileBytes / 512 * 512);
+          }
+        }
+        held = (held << 1) | (blk >= 0 ? 1u : 0u);
+        cp_async_commit();
+      };
 #pragma unroll
-          for (int a = 0; a < NG; ++a) {
-            float acc[NT][4];
+      for (int i = 0; i < kDq4Stages - 1; ++i) issue(i);
+      for (int i = 0; i < cnt; ++i) {
+        cp_async_wait<kDq4Stages - 2>();
+        __syncwarp();  // every lane's pieces are in, and the tile before is read by all
+        issue(i + kDq4Stages - 1);
+        if (((held >> (kDq4Stages - 1)) & 1u) == 0) continue;  // a page outside the cache holds no keys
+        const uint8_t* tile = sm.ring[warp] + (i % kDq4Stages) * L::kTileBytes;
+        const int left = len - 16 * (first + kDq4Warps * i);
+        const bool in0 = 2 * g < left, in1 = 2 * g + 1 < left;
+        uint32_t prm[2][2 * NG];  // of tokens 2g, 2g+1: K (s, lo) of each group, then V
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+        for (int e = 0; e < 2; ++e) {
+          const uint8_t* pp = tile + L::kParamOff + (2 * g + e) * L::kTokenParams;
+          if constexpr (NG == 2) {
+            const uint4 v = *reinterpret_cast<const uint4*>(pp);
+            prm[e][0] = v.x; prm[e][1] = v.y; prm[e][2] = v.z; prm[e][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(pp);
+            prm[e][0] = v.x; prm[e][1] = v.y;
+          }
+        }
+        if (left < 16) {  // keys past the end: unwritten bytes may be anything
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t w0 = fr.k[0][2 * a + e], w1 = fr.k[1][2 * a + e];
-              const uint32_t fa[4] = {q4_pair<F16, 0>(w0), q4_pair<F16, 0>(w1), q4_pair<F16, 1>(w0), q4_pair<F16, 1>(w1)};
-              const uint32_t fb[4] = {q4_pair<F16, 2>(w0), q4_pair<F16, 2>(w1), q4_pair<F16, 3>(w0), q4_pair<F16, 3>(w1)};
+          for (int a = 0; a < 2 * NG; ++a) {
+            prm[0][a] = in0 ? prm[0][a] : 0u;
+            prm[1][a] = in1 ? prm[1][a] : 0u;
+          }
+        }
+        // ---- scores: rows are tokens 2g (c0, c1) and 2g+1 (c2, c3)
+        uint32_t kw[2][KW];
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816<F16>(acc[nt], fa, qb[nt][2 * (2 * a + e)][0], qb[nt][2 * (2 * a + e)][1]);
-                mma16816<F16>(acc[nt], fb, qb[nt][2 * (2 * a + e) + 1][0], qb[nt][2 * (2 * a + e) + 1][1]);
-              }
-            }
-            const float s0 = q4_up<F16>(fr.prm[0][a] & 0xffffu), z0 = fmaf(8.f, s0, q4_up<F16>(fr.prm[0][a] >> 16));
-            const float s1 = q4_up<F16>(fr.prm[1][a] & 0xffffu), z1 = fmaf(8.f, s1, q4_up<F16>(fr.prm[1][a] >> 16));
+        for (int e = 0; e < 2; ++e) {
+          const uint8_t* kp = tile + (2 * g + e) * (D / 2) + t * (D / 8);
+          if constexpr (NG == 2) {
+            const uint4 v = *reinterpret_cast<const uint4*>(kp);
+            kw[e][0] = v.x; kw[e][1] = v.y; kw[e][2] = v.z; kw[e][3] = v.w;
+          } else {
+            const uint2 v = *reinterpret_cast<const uint2*>(kp);
+            kw[e][0] = v.x; kw[e][1] = v.y;
+          }
+        }
+        float sc[NT][4];
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          float acc[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t w0 = kw[0][2 * a + e], w1 = kw[1][2 * a + e];
+            const uint32_t fa[4] = {q4_pair16<F16, 0>(w0), q4_pair16<F16, 0>(w1), q4_pair16<F16, 1>(w0), q4_pair16<F16, 1>(w1)};
+            const uint32_t fb[4] = {q4_pair16<F16, 2>(w0), q4_pair16<F16, 2>(w1), q4_pair16<F16, 3>(w0), q4_pair16<F16, 3>(w1)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              sc[nt][0] += fmaf(s0, acc[nt][0], z0 * sq[nt][a][0]);
-              sc[nt][1] += fmaf(s0, acc[nt][1], z0 * sq[nt][a][1]);
-              sc[nt][2] += fmaf(s1, acc[nt][2], z1 * sq[nt][a][0]);
-              sc[nt][3] += fmaf(s1, acc[nt][3], z1 * sq[nt][a][1]);
+              mma16816<F16>(acc[nt], fa, qb[nt][2 * (2 * a + e)][0], qb[nt][2 * (2 * a + e)][1]);
+              mma16816<F16>(acc[nt], fb, qb[nt][2 * (2 * a + e) + 1][0], qb[nt][2 * (2 * a + e) + 1][1]);
             }
           }
-          bool raise = false;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[nt][e] = ((e < 2) ? in0 : in1) ? sc[nt][e] * p.scale_log2 : -INFINITY;
-            raise = raise || fmaxf(sc[nt][0], sc[nt][2]) > m_run[nt][0] + kRescaleThreshold ||
-                    fmaxf(sc[nt][1], sc[nt][3]) > m_run[nt][1] + kRescaleThreshold;
-          }
-          if (__any_sync(0xffffffffu, raise)) {
-            // the running base is only raised when a score exceeds it by 8 (p <= 2^8)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float mx = fmaxf(sc[nt][e], sc[nt][e + 2]);
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                const float m_new = fmaxf(m_run[nt][e], mx);
-                const float al = m_new == -INFINITY ? 1.f : ex2_approx(m_run[nt][e] - m_new);
-                m_run[nt][e] = m_new;
-                l_run[nt][e] *= al;
-#pragma unroll
-                for (int a = 0; a < NG; ++a) {
-                  vz[nt][a][e] *= al;
-#pragma unroll
-                  for (int i2 = 0; i2 < 4; ++i2) {
-                    o[nt][a][i2][e] *= al;
-                    o[nt][a][i2][e + 2] *= al;
-                  }
-                }
-              }
-          }
-          float pr[NT][4];
+          const float s0 = q4_up<F16>(prm[0][a] & 0xffffu), z0 = fmaf(-16.f, s0, q4_up<F16>(prm[0][a] >> 16));
+          const float s1 = q4_up<F16>(prm[1][a] & 0xffffu), z1 = fmaf(-16.f, s1, q4_up<F16>(prm[1][a] >> 16));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float base = m_run[nt][e & 1] == -INFINITY ? 0.f : m_run[nt][e & 1];
-              pr[nt][e] = ex2_approx(sc[nt][e] - base);
+              const float base = a == 0 ? 0.f : sc[nt][e];
+              sc[nt][e] = fmaf(e < 2 ? z0 : z1, sq[nt][a][e & 1], fmaf(e < 2 ? s0 : s1, acc[nt][e], base));
             }
-            l_run[nt][0] += pr[nt][0] + pr[nt][2];
-            l_run[nt][1] += pr[nt][1] + pr[nt][3];
           }
-          // ---- O += V^T P per group
+        }
+        bool raise = false;
 #pragma unroll
-          for (int a = 0; a < NG; ++a) {
-            const float s0 = q4_up<F16>(fr.prm[0][NG + a] & 0xffffu), s1 = q4_up<F16>(fr.prm[1][NG + a] & 0xffffu);
-            const float z0 = fmaf(8.f, s0, q4_up<F16>(fr.prm[0][NG + a] >> 16));
-            const float z1 = fmaf(8.f, s1, q4_up<F16>(fr.prm[1][NG + a] >> 16));
-            uint32_t bh[NT][2], bl[NT][2];
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[nt][e] *= p.scale_log2;
+          if (left < 16) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[nt][e] = (e < 2 ? in0 : in1) ? sc[nt][e] : -INFINITY;
+          }
+          raise = raise || fmaxf(sc[nt][0], sc[nt][2]) > limit[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > limit[nt][1];
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+          // the base is only raised when a score exceeds it by 8 (weights <= 2^8)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(sc[nt][e], sc[nt][e + 2]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float old = limit[nt][e] - kRescaleThreshold;
+              limit[nt][e] = fmaxf(old, mx) + kRescaleThreshold;
+              const float now = limit[nt][e] - kRescaleThreshold;  // rounded as it is used
+              const float al = now == -INFINITY ? 1.f : ex2_approx(old - now);
+              l_run[nt][e] *= al;
+#pragma unroll
+              for (int a = 0; a < NG; ++a) {
+                vz[nt][a][e] *= al;
+#pragma unroll
+                for (int i2 = 0; i2 < 4; ++i2) {
+                  o[nt][a][i2][e] *= al;
+                  o[nt][a][i2][e + 2] *= al;
+                }
+              }
+            }
+        }
+        float pr[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float base = limit[nt][e & 1] == -INFINITY ? 0.f : limit[nt][e & 1] - kRescaleThreshold;
+            pr[nt][e] = ex2_approx(sc[nt][e] - base);
+          }
+          l_run[nt][0] += pr[nt][0] + pr[nt][2];
+          l_run[nt][1] += pr[nt][1] + pr[nt][3];
+        }
+        // ---- O += V^T P per group
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          const uint4 vw = *reinterpret_cast<const uint4*>(tile + L::kVOff + (a * 8 + g) * 64 + t * 16);
+          const uint32_t vwords[4] = {vw.x, vw.y, vw.z, vw.w};
+          const float s0 = q4_up<F16>(prm[0][NG + a] & 0xffffu), s1 = q4_up<F16>(prm[1][NG + a] & 0xffffu);
+          const float z0 = fmaf(8.f, s0, q4_up<F16>(prm[0][NG + a] >> 16));
+          const float z1 = fmaf(8.f, s1, q4_up<F16>(prm[1][NG + a] >> 16));
+          uint32_t bh[NT][2], bl[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            vz[nt][a][0] = fmaf(pr[nt][0], z0, fmaf(pr[nt][2], z1, vz[nt][a][0]));
+            vz[nt][a][1] = fmaf(pr[nt][1], z0, fmaf(pr[nt][3], z1, vz[nt][a][1]));
+            const float x0 = pr[nt][0] * s0, x1 = pr[nt][1] * s0, x2 = pr[nt][2] * s1, x3 = pr[nt][3] * s1;
+            const uint32_t h0 = pack2<false>(x0, x1), h1 = pack2<false>(x2, x3);
+            const float2 u0 = unpack2<false>(h0), u1 = unpack2<false>(h1);
+            const uint32_t l0 = pack2<false>(x0 - u0.x, x1 - u0.y), l1 = pack2<false>(x2 - u1.x, x3 - u1.y);
+            bh[nt][0] = movmatrix_t(h0);
+            bh[nt][1] = movmatrix_t(h1);
+            bl[nt][0] = movmatrix_t(l0);
+            bl[nt][1] = movmatrix_t(l1);
+          }
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) {
+            const uint32_t w = vwords[i2];
+            const uint32_t fa[4] = {q4_pair_centred<0>(w), q4_pair_centred<1>(w), q4_pair_centred<2>(w), q4_pair_centred<3>(w)};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              vz[nt][a][0] += fmaf(pr[nt][0], z0, pr[nt][2] * z1);
-              vz[nt][a][1] += fmaf(pr[nt][1], z0, pr[nt][3] * z1);
-              const float x0 = pr[nt][0] * s0, x1 = pr[nt][1] * s0, x2 = pr[nt][2] * s1, x3 = pr[nt][3] * s1;
-              const uint32_t h0 = pack2<false>(x0, x1), h1 = pack2<false>(x2, x3);
-              const float2 u0 = unpack2<false>(h0), u1 = unpack2<false>(h1);
-              const uint32_t l0 = pack2<false>(x0 - u0.x, x1 - u0.y), l1 = pack2<false>(x2 - u1.x, x3 - u1.y);
-              bh[nt][0] = movmatrix_t(h0);
-              bh[nt][1] = movmatrix_t(h1);
-              bl[nt][0] = movmatrix_t(l0);
-              bl[nt][1] = movmatrix_t(l1);
-            }
-#pragma unroll
-            for (int i2 = 0; i2 < 4; ++i2) {
-              const uint32_t w = fr.v[a][i2];
-              const uint32_t fa[4] = {q4_pair<false, 0>(w), q4_pair<false, 1>(w), q4_pair<false, 2>(w), q4_pair<false, 3>(w)};
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma16816<false>(o[nt][a][i2], fa, bh[nt][0], bh[nt][1]);
-                mma16816<false>(o[nt][a][i2], fa, bl[nt][0], bl[nt][1]);
-              }
+              mma16816<false>(o[nt][a][i2], fa, bh[nt][0], bh[nt][1]);
+              mma16816<false>(o[nt][a][i2], fa, bl[nt][0], bl[nt][1]);
             }
           }
         }
       }
+      cp_async_wait<0>();
+      __syncthreads();  // the rings are read: their memory takes the sums
 
       // ---- join the warps: sums over the lanes' tokens first
 #pragma unroll
@@ -425,7 +452,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
           for (int s = 4; s < 32; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
           const int col = nt * 8 + 2 * t + e;
           if (g == 0) {
-            sm.m[warp][col] = l != l ? 0.f : m_run[nt][e];  // a NaN sum must not hide behind an empty base
+            sm.m[warp][col] = l != l ? 0.f : limit[nt][e] - kRescaleThreshold;  // a NaN sum must not hide behind an empty base
             sm.l[warp][col] = l;
           }
 #pragma unroll

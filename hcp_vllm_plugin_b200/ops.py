@@ -7,6 +7,7 @@ attention: there is no CPU path.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import NamedTuple
 
@@ -21,6 +22,8 @@ _DT = {torch.bfloat16: C.HCP_BF16, torch.float16: C.HCP_F16, torch.float32: C.HC
 #   q_start, q_len, paged_req, lse_col, then per segment (src, start, len, causal_off) x 2
 WORK_FIELDS = 12
 
+_HERE = contextlib.nullcontext()  # the tensor's GPU is the current one already
+
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
@@ -28,15 +31,18 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _rows_heads(t: torch.Tensor, name: str) -> int:
     """Row stride (elements) of a [rows, heads, D] tensor whose last two dims are packed."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(t.shape)}")
-    if t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3:
+        raise ValueError(f"{name} must be [rows, heads, head_dim], got {tuple(shape)}")
+    rows, heads, d = shape
+    if stride[2] != 1 or stride[1] != d:
         raise ValueError(f"{name} must be contiguous in its last two dims")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+    return stride[0] if rows > 1 else heads * d
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    # the handle alone: a Stream object costs as much as a launch
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def _same_device(ref: torch.Tensor, **tensors) -> None:
@@ -54,7 +60,7 @@ def _same_device(ref: torch.Tensor, **tensors) -> None:
 def _dev(t: torch.Tensor):
     """Make the tensor's GPU the current device for the library call: the
     library launches on the current device, into a stream of that device."""
-    return torch.cuda.device(t.device)
+    return _HERE if torch.cuda.current_device() == t.get_device() else torch.cuda.device(t.device)
 
 
 def _ext_sources(ext, dtype, ref: torch.Tensor):
@@ -494,13 +500,18 @@ def kv_plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     dev = context_lens.device
     wide = torch.empty(2 * num_tokens, dtype=torch.int64, device=dev)
     small = torch.empty(2 * reqs + 2 * num_tokens + 3, dtype=torch.int32, device=dev)
-    positions, slots = wide.split([num_tokens, num_tokens])
-    start, lens, req, kv, head, missing = small.split([reqs + 1, reqs, num_tokens, num_tokens, 1, 1])
-    a.query_start, a.seq_lens, a.positions, a.slot_mapping = _ptr(start), _ptr(lens), _ptr(positions), _ptr(slots)
-    a.token_req, a.kv_lens, a.free_head_out, a.missing_out = _ptr(req), _ptr(kv), _ptr(head), _ptr(missing)
+    at, at64 = _ptr(small), _ptr(wide)
+    a.positions, a.slot_mapping = at64, at64 + 8 * num_tokens
+    a.query_start, a.seq_lens = at, at + 4 * (reqs + 1)
+    a.token_req = at + 4 * (2 * reqs + 1)
+    a.kv_lens = a.token_req + 4 * num_tokens
+    a.free_head_out, a.missing_out = a.kv_lens + 4 * num_tokens, a.kv_lens + 4 * num_tokens + 4
     a.num_reqs, a.block_size, a.num_tokens = reqs, int(block_size), int(num_tokens)
     with _dev(context_lens):
         C.check(C.load().hcp_kv_plan_step(ctypes.byref(a), _stream(context_lens)), "hcp_kv_plan_step")
+    # the views are made while the kernel runs
+    positions, slots = wide.split_with_sizes([num_tokens, num_tokens])
+    start, lens, req, kv, head, missing = small.split_with_sizes([reqs + 1, reqs, num_tokens, num_tokens, 1, 1])
     return KvStepPlan(start, lens, positions, slots, req, kv, head, missing)
 
 
