@@ -7,19 +7,23 @@
 //
 // Bound by HBM: 9/8 D bytes per key and KV head (K and V), against 2 G D
 // products.  What has to be kept small is the work per byte.  So:
-//   * the whole numbers n are the matrix operands, exact in 16 bits; scales and
-//     lowest values are applied outside, per 64-dim group:
+//   * the whole numbers n - 8 are the matrix operands, exact in fp16; scales and
+//     lowest values are applied outside in 32 bits, per 64-dim group:
 //       q . k  = sum_g  s_g (q_g . (n_g - 8)) + (lo_g + 8 s_g) sum(q_g)
 //       o_g    = sum_j (p_j s_j) (n_j - 8)    + sum_j p_j (lo_j + 8 s_j)
-//     (n - 8 keeps the accumulated sums as small as the result's own terms);
+//     (centred, the accumulated sums stay as small as the result's own terms);
 //   * keys are the rows of the first product (16 keys x 8 heads) and dims those of
 //     the second (16 dims x 8 heads), so a group of up to 8 query heads fills the
 //     instruction's 8 columns instead of half of 16 rows;
 //   * the tile layout gives every lane its fragments of both products in whole
 //     16-byte pieces: no shared memory, no transposes; only the 8 x 8 blocks of P
 //     are transposed between the products (movmatrix);
-//   * p_j s_j enters the second product as a bf16 high part and the rest (two
-//     products), ~16 significant bits; bf16 whatever the rows' type, for its range.
+//   * q and p_j s_j enter the products in fp16, scaled by powers of two: q by its
+//     head's largest element (no loss), p_j s_j by the largest scale met so far.
+//     Rounding p_j s_j to 11 bits is off by at most 2^-11 of each key's term, and the
+//     terms' weights sum to one: a quarter of what rounding the result to bf16 may be
+//     off.  A second product for the rest costs 8 of the 16 matrix instructions and
+//     a tenth of the issue slots of a kernel that is bound by them.
 //
 // Split: all rows' tiles of 16 keys, heads outermost in a row, form one line that
 // the blocks cut into equal pieces, so any mix of lengths is even and nothing
@@ -88,20 +92,21 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   return d;
 }
 
-// Nibbles I and I+4 of a word as a pair 16 + n in 16 bits: the nibble becomes the
-// upper mantissa bits of 16.
-template <bool F16, int I>
-__device__ __forceinline__ uint32_t q4_pair16(uint32_t w) {
-  constexpr int kAt = F16 ? 6 : 3;  // lowest mantissa bit that counts 1
-  const uint32_t v = 4 * I > kAt ? w >> (4 * I > kAt ? 4 * I - kAt : 0) : w << (4 * I > kAt ? 0 : kAt - 4 * I);
-  return F16 ? (v & 0x03c003c0u) | 0x4c004c00u : (v & 0x00780078u) | 0x41804180u;
-}
-// ... and as a pair n - 8 in bf16: 128 + n from the lowest mantissa bits, minus 136 (exact).
-template <int I>
-__device__ __forceinline__ uint32_t q4_pair_centred(uint32_t w) {
-  const uint32_t v = ((w >> (4 * I)) & 0x000f000fu) | 0x43004300u;
-  const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&v), __floats2bfloat162_rn(136.f, 136.f));
-  return *reinterpret_cast<const uint32_t*>(&r);
+// Whole numbers of a word's nibbles I and I+4 as a pair n - 8 in fp16, exact.  With a
+// nibble in mantissa bits 0-3 of 1024 the value is 1024 + n, in bits 4-7 it is
+// 1024 + 16 n: two pairs without a shift, the other two after one shift by 8.
+__device__ __forceinline__ void q4_pairs(uint32_t w, uint32_t (&r)[4]) {
+  const __half2 c0 = __floats2half2_rn(-1032.f, -1032.f), c1 = __floats2half2_rn(-72.f, -72.f);
+  const __half2 sixteenth = __floats2half2_rn(0.0625f, 0.0625f);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t v = i == 0 ? w : w >> 8;
+    const uint32_t a = (v & 0x000f000fu) | 0x64006400u, b = (v & 0x00f000f0u) | 0x64006400u;
+    const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&a), c0);
+    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, c1);
+    r[2 * i] = *reinterpret_cast<const uint32_t*>(&x);
+    r[2 * i + 1] = *reinterpret_cast<const uint32_t*>(&y);
+  }
 }
 
 // Tiles of a row (0 for a padding row or an empty one).
@@ -204,30 +209,50 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
       const int t0 = static_cast<int>((f - cum) - static_cast<long long>(kvh) * tiles);
       const int n = static_cast<int>(min(static_cast<long long>(tiles - t0), f_end - f));
 
-      // ---- Q fragments: columns are heads, lane's k index pairs (d, d + 4)
+      // ---- Q fragments: columns are heads, lane's k index pairs (d, d + 4).  Each head is
+      // scaled by a power of two to the top of fp16's range and rounded to it: exact down to
+      // 2^-29 of its largest element for 11-bit elements.  The power goes into the head's factor.
       uint32_t qb[NT][2 * KW][2];
-      float sq[NT][NG][2];  // sums of q over each group, heads 2t and 2t+1
+      float sq[NT][NG][2];  // sums of the scaled q over each group, heads 2t and 2t+1
+      float hs[NT][2];      // score = hs * (scaled q . k), in log2 units
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int hc = nt * 8 + g;
         const uint16_t* qh = static_cast<const uint16_t*>(p.q) + row * p.q_row_stride +
                              static_cast<long long>(kvh * G + hc) * D;
+        uint4 raw[KW];
+        float top = 0.f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) {
+          raw[w] = make_uint4(0u, 0u, 0u, 0u);
+          if (hc < G) raw[w] = *reinterpret_cast<const uint4*>(qh + 64 * (w >> 1) + 16 * t + 8 * (w & 1));
+          float x[8];
+          q4_unpack8<F16>(raw[w], x);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // 2^e with top * 2^e in [2^14, 2^15), e at most 126 (and 0 for an empty or infinite head)
+        const int ex = static_cast<int>(__float_as_uint(top) >> 23);
+        const int e = ex == 0 || ex == 255 ? 0 : min(126, 141 - ex);
+        const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
         float part[NG];
 #pragma unroll
         for (int a = 0; a < NG; ++a) part[a] = 0.f;
 #pragma unroll
         for (int w = 0; w < KW; ++w) {
-          const int grp = w >> 1;
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (hc < G) v = *reinterpret_cast<const uint4*>(qh + 64 * grp + 16 * t + 8 * (w & 1));
-          qb[nt][2 * w][0] = __byte_perm(v.x, v.z, 0x5410);      // d, d+4
-          qb[nt][2 * w][1] = __byte_perm(v.x, v.z, 0x7632);      // d+1, d+5
-          qb[nt][2 * w + 1][0] = __byte_perm(v.y, v.w, 0x5410);  // d+2, d+6
-          qb[nt][2 * w + 1][1] = __byte_perm(v.y, v.w, 0x7632);  // d+3, d+7
           float x[8];
-          q4_unpack8<F16>(v, x);
+          q4_unpack8<F16>(raw[w], x);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) part[grp] += x[i];
+          for (int i = 0; i < 8; ++i) {
+            x[i] *= up;
+            part[w >> 1] += x[i];
+          }
+          qb[nt][2 * w][0] = pack2<true>(x[0], x[4]);
+          qb[nt][2 * w][1] = pack2<true>(x[1], x[5]);
+          qb[nt][2 * w + 1][0] = pack2<true>(x[2], x[6]);
+          qb[nt][2 * w + 1][1] = pack2<true>(x[3], x[7]);
         }
 #pragma unroll
         for (int a = 0; a < NG; ++a) {
@@ -236,10 +261,22 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
           sq[nt][a][0] = __shfl_sync(0xffffffffu, part[a], 8 * t);
           sq[nt][a][1] = __shfl_sync(0xffffffffu, part[a], 8 * t + 4);
         }
+        const float down = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+        hs[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
+        hs[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
       }
       float o[NT][NG][4][4];
       float vz[NT][NG][2], l_run[NT][2];
-      float limit[NT][2];  // base of the weights + 8; the base is the running maximum or up to 8 below it
+      float base[NT][2];   // of the weights: the running maximum or up to 8 below it; -inf before the first key
+      float limit[NT][2];  // the score / hs at which the base has to rise: (base + 8) / hs
+      float vref[NG];      // powers of two: the sums o are in units of vref, 1 / vref multiplies V's scales
+      float vinv[NG], vlim[NG];
+#pragma unroll
+      for (int a = 0; a < NG; ++a) {
+        vref[a] = 0.f;
+        vinv[a] = 0.f;
+        vlim[a] = 0.f;
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -248,7 +285,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
 #pragma unroll
           for (int i = 0; i < 4; ++i) o[nt][a][i][0] = o[nt][a][i][1] = o[nt][a][i][2] = o[nt][a][i][3] = 0.f;
         }
-        limit[nt][0] = limit[nt][1] = -INFINITY;
+        limit[nt][0] = limit[nt][1] = base[nt][0] = base[nt][1] = -INFINITY;
         l_run[nt][0] = l_run[nt][1] = 0.f;
       }
 
@@ -296,39 +333,30 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
         if (((held >> (kDq4Stages - 1)) & 1u) == 0) continue;  // a page outside the cache holds no keys
         const uint8_t* tile = sm.ring[warp] + (i % kDq4Stages) * L::kTileBytes;
         const int left = len - 16 * (first + kDq4Warps * i);
-        const bool in0 = 2 * g < left, in1 = 2 * g + 1 < left;
         uint32_t prm[2][2 * NG];  // of tokens 2g, 2g+1: K (s, lo) of each group, then V
+        uint32_t kw[2][KW];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const uint8_t* pp = tile + L::kParamOff + (2 * g + e) * L::kTokenParams;
+          const uint8_t* kp = tile + (2 * g + e) * (D / 2) + t * (D / 8);
           if constexpr (NG == 2) {
-            const uint4 v = *reinterpret_cast<const uint4*>(pp);
+            const uint4 v = *reinterpret_cast<const uint4*>(pp), u = *reinterpret_cast<const uint4*>(kp);
             prm[e][0] = v.x; prm[e][1] = v.y; prm[e][2] = v.z; prm[e][3] = v.w;
+            kw[e][0] = u.x; kw[e][1] = u.y; kw[e][2] = u.z; kw[e][3] = u.w;
           } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(pp);
+            const uint2 v = *reinterpret_cast<const uint2*>(pp), u = *reinterpret_cast<const uint2*>(kp);
             prm[e][0] = v.x; prm[e][1] = v.y;
+            kw[e][0] = u.x; kw[e][1] = u.y;
           }
         }
         if (left < 16) {  // keys past the end: unwritten bytes may be anything
 #pragma unroll
           for (int a = 0; a < 2 * NG; ++a) {
-            prm[0][a] = in0 ? prm[0][a] : 0u;
-            prm[1][a] = in1 ? prm[1][a] : 0u;
+            prm[0][a] = 2 * g < left ? prm[0][a] : 0u;
+            prm[1][a] = 2 * g + 1 < left ? prm[1][a] : 0u;
           }
         }
         // ---- scores: rows are tokens 2g (c0, c1) and 2g+1 (c2, c3)
-        uint32_t kw[2][KW];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint8_t* kp = tile + (2 * g + e) * (D / 2) + t * (D / 8);
-          if constexpr (NG == 2) {
-            const uint4 v = *reinterpret_cast<const uint4*>(kp);
-            kw[e][0] = v.x; kw[e][1] = v.y; kw[e][2] = v.z; kw[e][3] = v.w;
-          } else {
-            const uint2 v = *reinterpret_cast<const uint2*>(kp);
-            kw[e][0] = v.x; kw[e][1] = v.y;
-          }
-        }
         float sc[NT][4];
 #pragma unroll
         for (int a = 0; a < NG; ++a) {
@@ -337,39 +365,44 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
           for (int nt = 0; nt < NT; ++nt) acc[nt][0] = acc[nt][1] = acc[nt][2] = acc[nt][3] = 0.f;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t w0 = kw[0][2 * a + e], w1 = kw[1][2 * a + e];
-            const uint32_t fa[4] = {q4_pair16<F16, 0>(w0), q4_pair16<F16, 0>(w1), q4_pair16<F16, 1>(w0), q4_pair16<F16, 1>(w1)};
-            const uint32_t fb[4] = {q4_pair16<F16, 2>(w0), q4_pair16<F16, 2>(w1), q4_pair16<F16, 3>(w0), q4_pair16<F16, 3>(w1)};
+            uint32_t x[4], y[4];
+            q4_pairs(kw[0][2 * a + e], x);
+            q4_pairs(kw[1][2 * a + e], y);
+            const uint32_t fa[4] = {x[0], y[0], x[1], y[1]}, fb[4] = {x[2], y[2], x[3], y[3]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-              mma16816<F16>(acc[nt], fa, qb[nt][2 * (2 * a + e)][0], qb[nt][2 * (2 * a + e)][1]);
-              mma16816<F16>(acc[nt], fb, qb[nt][2 * (2 * a + e) + 1][0], qb[nt][2 * (2 * a + e) + 1][1]);
+              mma16816<true>(acc[nt], fa, qb[nt][2 * (2 * a + e)][0], qb[nt][2 * (2 * a + e)][1]);
+              mma16816<true>(acc[nt], fb, qb[nt][2 * (2 * a + e) + 1][0], qb[nt][2 * (2 * a + e) + 1][1]);
             }
           }
-          const float s0 = q4_up<F16>(prm[0][a] & 0xffffu), z0 = fmaf(-16.f, s0, q4_up<F16>(prm[0][a] >> 16));
-          const float s1 = q4_up<F16>(prm[1][a] & 0xffffu), z1 = fmaf(-16.f, s1, q4_up<F16>(prm[1][a] >> 16));
+          const float s0 = q4_up<F16>(prm[0][a] & 0xffffu), z0 = fmaf(8.f, s0, q4_up<F16>(prm[0][a] >> 16));
+          const float s1 = q4_up<F16>(prm[1][a] & 0xffffu), z1 = fmaf(8.f, s1, q4_up<F16>(prm[1][a] >> 16));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float base = a == 0 ? 0.f : sc[nt][e];
-              sc[nt][e] = fmaf(e < 2 ? z0 : z1, sq[nt][a][e & 1], fmaf(e < 2 ? s0 : s1, acc[nt][e], base));
-            }
+            for (int e = 0; e < 4; ++e)
+              sc[nt][e] = fmaf(e < 2 ? z0 : z1, sq[nt][a][e & 1], fmaf(e < 2 ? s0 : s1, acc[nt][e], a == 0 ? 0.f : sc[nt][e]));
           }
+        }
+        if (left < 16) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sc[nt][e] = 2 * g + (e >> 1) < left ? sc[nt][e] : -INFINITY;
         }
         bool raise = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sc[nt][e] *= p.scale_log2;
-          if (left < 16) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sc[nt][e] = (e < 2 ? in0 : in1) ? sc[nt][e] : -INFINITY;
-          }
+        for (int nt = 0; nt < NT; ++nt)
           raise = raise || fmaxf(sc[nt][0], sc[nt][2]) > limit[nt][0] || fmaxf(sc[nt][1], sc[nt][3]) > limit[nt][1];
+        float vs[2][NG];
+#pragma unroll
+        for (int a = 0; a < NG; ++a) {
+          vs[0][a] = q4_up<F16>(prm[0][NG + a] & 0xffffu);
+          vs[1][a] = q4_up<F16>(prm[1][NG + a] & 0xffffu);
+          raise = raise || fmaxf(vs[0][a], vs[1][a]) > vlim[a];
         }
         if (__any_sync(0xffffffffu, raise)) {
-          // the base is only raised when a score exceeds it by 8 (weights <= 2^8)
+          // a score above the base by more than 8 raises it (weights <= 2^8)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -378,10 +411,10 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
               mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float old = limit[nt][e] - kRescaleThreshold;
-              limit[nt][e] = fmaxf(old, mx) + kRescaleThreshold;
-              const float now = limit[nt][e] - kRescaleThreshold;  // rounded as it is used
-              const float al = now == -INFINITY ? 1.f : ex2_approx(old - now);
+              const float now = fmaxf(base[nt][e], mx * hs[nt][e]);
+              const float al = now == -INFINITY ? 1.f : ex2_approx(base[nt][e] - now);
+              base[nt][e] = now;
+              limit[nt][e] = now == -INFINITY ? -INFINITY : __fdividef(now + kRescaleThreshold, hs[nt][e]);
               l_run[nt][e] *= al;
 #pragma unroll
               for (int a = 0; a < NG; ++a) {
@@ -393,15 +426,38 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
                 }
               }
             }
+          // a scale above 2^7 vref raises vref: weight times scale stays below 2^15 in fp16
+#pragma unroll
+          for (int a = 0; a < NG; ++a) {
+            float mx = fmaxf(vs[0][a], vs[1][a]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            if (mx > vlim[a]) {
+              // 2^6 vref <= mx < 2^7 vref now (vref and 1 / vref stay normal numbers)
+              const int ex = max(static_cast<int>(__float_as_uint(mx) >> 23) - 6, 1);
+              const float now = __uint_as_float(static_cast<uint32_t>(ex) << 23);
+              const float al = vref[a] * __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+              vref[a] = now;
+              vinv[a] = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
+              vlim[a] = now * 128.f;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int i2 = 0; i2 < 4; ++i2)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) o[nt][a][i2][e] *= al;
+            }
+          }
         }
         float pr[NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float base = limit[nt][e & 1] == -INFINITY ? 0.f : limit[nt][e & 1] - kRescaleThreshold;
-            pr[nt][e] = ex2_approx(sc[nt][e] - base);
-          }
+          const float b0 = base[nt][0] == -INFINITY ? 0.f : base[nt][0], b1 = base[nt][1] == -INFINITY ? 0.f : base[nt][1];
+          pr[nt][0] = ex2_approx(fmaf(sc[nt][0], hs[nt][0], -b0));
+          pr[nt][1] = ex2_approx(fmaf(sc[nt][1], hs[nt][1], -b1));
+          pr[nt][2] = ex2_approx(fmaf(sc[nt][2], hs[nt][0], -b0));
+          pr[nt][3] = ex2_approx(fmaf(sc[nt][3], hs[nt][1], -b1));
           l_run[nt][0] += pr[nt][0] + pr[nt][2];
           l_run[nt][1] += pr[nt][1] + pr[nt][3];
         }
@@ -410,32 +466,23 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
         for (int a = 0; a < NG; ++a) {
           const uint4 vw = *reinterpret_cast<const uint4*>(tile + L::kVOff + (a * 8 + g) * 64 + t * 16);
           const uint32_t vwords[4] = {vw.x, vw.y, vw.z, vw.w};
-          const float s0 = q4_up<F16>(prm[0][NG + a] & 0xffffu), s1 = q4_up<F16>(prm[1][NG + a] & 0xffffu);
-          const float z0 = fmaf(8.f, s0, q4_up<F16>(prm[0][NG + a] >> 16));
-          const float z1 = fmaf(8.f, s1, q4_up<F16>(prm[1][NG + a] >> 16));
-          uint32_t bh[NT][2], bl[NT][2];
+          const float z0 = fmaf(8.f, vs[0][a], q4_up<F16>(prm[0][NG + a] >> 16));
+          const float z1 = fmaf(8.f, vs[1][a], q4_up<F16>(prm[1][NG + a] >> 16));
+          const float s0 = vs[0][a] * vinv[a], s1 = vs[1][a] * vinv[a];
+          uint32_t bp[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             vz[nt][a][0] = fmaf(pr[nt][0], z0, fmaf(pr[nt][2], z1, vz[nt][a][0]));
             vz[nt][a][1] = fmaf(pr[nt][1], z0, fmaf(pr[nt][3], z1, vz[nt][a][1]));
-            const float x0 = pr[nt][0] * s0, x1 = pr[nt][1] * s0, x2 = pr[nt][2] * s1, x3 = pr[nt][3] * s1;
-            const uint32_t h0 = pack2<false>(x0, x1), h1 = pack2<false>(x2, x3);
-            const float2 u0 = unpack2<false>(h0), u1 = unpack2<false>(h1);
-            const uint32_t l0 = pack2<false>(x0 - u0.x, x1 - u0.y), l1 = pack2<false>(x2 - u1.x, x3 - u1.y);
-            bh[nt][0] = movmatrix_t(h0);
-            bh[nt][1] = movmatrix_t(h1);
-            bl[nt][0] = movmatrix_t(l0);
-            bl[nt][1] = movmatrix_t(l1);
+            bp[nt][0] = movmatrix_t(pack2<true>(pr[nt][0] * s0, pr[nt][1] * s0));
+            bp[nt][1] = movmatrix_t(pack2<true>(pr[nt][2] * s1, pr[nt][3] * s1));
           }
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
-            const uint32_t w = vwords[i2];
-            const uint32_t fa[4] = {q4_pair_centred<0>(w), q4_pair_centred<1>(w), q4_pair_centred<2>(w), q4_pair_centred<3>(w)};
+            uint32_t fa[4];  // dims 2p (row g) and 2p+1 (row g+8) of tokens 4t, 4t+2 and 4t+1, 4t+3
+            q4_pairs(vwords[i2], fa);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma16816<false>(o[nt][a][i2], fa, bh[nt][0], bh[nt][1]);
-              mma16816<false>(o[nt][a][i2], fa, bl[nt][0], bl[nt][1]);
-            }
+            for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][a][i2], fa, bp[nt][0], bp[nt][1]);
           }
         }
       }
@@ -452,7 +499,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
           for (int s = 4; s < 32; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
           const int col = nt * 8 + 2 * t + e;
           if (g == 0) {
-            sm.m[warp][col] = l != l ? 0.f : limit[nt][e] - kRescaleThreshold;  // a NaN sum must not hide behind an empty base
+            sm.m[warp][col] = l != l ? 0.f : base[nt][e];  // a NaN sum must not hide behind an empty base
             sm.l[warp][col] = l;
           }
 #pragma unroll
@@ -462,7 +509,7 @@ __global__ void __launch_bounds__(kDq4Threads, NT == 1 ? kDq4CtasPerSm : 2)
             for (int s = 4; s < 32; s <<= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
 #pragma unroll
             for (int i2 = 0; i2 < 4; ++i2) {
-              float2 v = make_float2(o[nt][a][i2][e] + z, o[nt][a][i2][e + 2] + z);
+              const float2 v = make_float2(fmaf(o[nt][a][i2][e], vref[a], z), fmaf(o[nt][a][i2][e + 2], vref[a], z));
               *reinterpret_cast<float2*>(&sm.o[warp][col][8 * (8 * a + g) + 2 * i2]) = v;
             }
           }

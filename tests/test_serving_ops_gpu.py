@@ -294,8 +294,10 @@ def _filled(ops, gen, nb, hkv, bs, d, dtype, scale=1.0):
 
 def _check_attention(got, lse, q, k, v, scale, dtype, what):
     """One row against 64 bits.  With a_i = scale * sum_d |q_d| max_j |k_jd| (i a head): a score is off by at most
-    2^-17 a_i (64 products summed in 32 bits per group, then the groups), so each weight by that and 2^-21 of ex2;
-    the weights' two 16-bit parts leave 2^-16; each of a tile's sums rounds by 2^-23, n / 16 tiles of them twice."""
+    2^-17 a_i (64 products summed in 32 bits per group, then the groups), so each weight by that and 2^-21 of ex2.
+    The products p_j s_j are rounded to fp16, half a step of 2^-10 off: 2^-11 p_j s_j |n_j - 8| of a result whose p_j
+    sum to 1.  |n - 8| <= 8, and 15 s <= 2 top (1 + 2^-8, s being rounded), so 8 s <= 1.08 top: 1.08 * 2^-11 top.
+    Each of a tile's sums rounds by 2^-23, n / 16 tiles of them twice."""
     n = k.shape[0]
     o, l = R.attention(q, k, v, scale)
     if n == 0:
@@ -305,9 +307,9 @@ def _check_attention(got, lse, q, k, v, scale, dtype, what):
     a = np.array([scale * (np.abs(q[i]) * np.abs(k[:, i // g]).max(0)).sum() for i in range(q.shape[0])])
     top = np.array([np.abs(v[:, i // g]).max() for i in range(q.shape[0])])
     dx = 2.0 ** -17 * a
-    slack = top * (2 * dx + 2.0 ** -15 + n / 8 * 2.0 ** -23)
+    slack = top * (2 * dx + 1.08 * 2.0 ** -11 + 2.0 ** -15 + n / 8 * 2.0 ** -23)
     eps = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
-    bar = slack[:, None] + eps * (np.abs(o) + slack[:, None]) + 2.0 ** -25
+    bar = slack[:, None] + eps * (np.abs(o) + slack[:, None]) + (2.0 ** -25 if dtype == torch.float16 else 0.0)
     assert (np.abs(got - o) <= bar).all(), (what, np.max(np.abs(got - o) / bar))
     assert (np.abs(lse - l) <= dx + 2.0 ** -20 * (np.abs(l) + 1) + n / 16 * 2.0 ** -24).all(), what
 
@@ -452,6 +454,29 @@ def test_decode_q4_extreme_scores(ops):
     q = _randn(gen, 2, h, d) * 4
     q[1] = 0
     _run_decode(ops, cache, q, [n, n - 3], torch.arange(nb, dtype=torch.int32).view(1, nb).repeat(2, 1), BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_decode_q4_scales_far_apart(ops, dtype):
+    """Values and queries whose size changes by powers of ten from token to token and head to head."""
+    gen = torch.Generator().manual_seed(14)
+    h, hkv, d, bs, nb = 14, 2, 128, 16, 30
+    n = nb * bs
+    v = torch.randn(n, hkv, d, generator=gen) * 10.0 ** torch.linspace(-4, 3, n)[:, None, None]
+    v[:, 1] = v[:, 1].flip(0)
+    v[40:60, :, :64] = 0.25     # groups without a range
+    cache = torch.zeros(ops.kv_cache_q4_shape(nb, hkv, bs, d), dtype=torch.uint8, device="cuda")
+    ops.kv_cache_update_q4(_randn(gen, n, hkv, d, dtype=dtype).cuda(), v.to(dtype).cuda(), cache, torch.arange(n, device="cuda"))
+    q = (torch.randn(3, h, d, generator=gen) * 10.0 ** torch.linspace(-4, 1, h)[:, None]).to(dtype)
+    table = torch.arange(nb, dtype=torch.int32).view(1, nb).repeat(3, 1)
+    _run_decode(ops, cache, q, [n, 200, 45], table, dtype)
+    # far past fp16's range either way, in bf16 (64 bits do not pass 10^38 either)
+    if dtype == BF16:
+        for size in (1e-30, 1e30):
+            ops.kv_cache_update_q4(_randn(gen, n, hkv, d).cuda(), (torch.randn(n, hkv, d, generator=gen) * size).to(dtype).cuda(), cache,
+                                   torch.arange(n, device="cuda"))
+            _run_decode(ops, cache, _randn(gen, 3, h, d), [n, 200, 45], table, dtype)
+            _run_decode(ops, cache, (torch.randn(3, h, d, generator=gen) * 1e-20).to(dtype), [n, 200, 45], table, dtype)
 
 
 def test_decode_q4_strided_rows_and_own_workspace(ops):
