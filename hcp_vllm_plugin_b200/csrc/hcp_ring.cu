@@ -943,21 +943,39 @@ int launch_norm_rope(const NormRopeParams& p, int64_t tokens, int kind, cudaStre
   return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }
 
+bool g_dq4_attr_done[2][2][2][64];
+
 template <int D, bool F16, int NT>
 int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
-  decode_q4_kernel<D, F16, NT><<<kDq4Ctas, kDq4Threads, 0, st>>>(p);
+  constexpr int smem = sizeof(Dq4Smem<D>);
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HCP_ERR_CUDA;
+  {
+    std::lock_guard<std::mutex> lk(g_attr_mu);
+    bool& done = g_dq4_attr_done[D == 128][F16][NT == 2][dev];
+    if (!done) {
+      if (cudaFuncSetAttribute(decode_q4_kernel<D, F16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return HCP_ERR_CUDA;
+      done = true;
+    }
+  }
+  decode_q4_kernel<D, F16, NT><<<kDq4Sms * dq4_ctas_per_sm(NT), kDq4Threads, smem, st>>>(p);
   if (cudaGetLastError() != cudaSuccess) return HCP_ERR_CUDA;
   // the joining kernel may start while the first one ends; it waits for it itself
+  const int64_t pairs = static_cast<int64_t>(p.rows) * p.num_kv_heads;
+  const bool share = pairs <= kDq4Sms;  // one pair or a few an SM: their parts are shared between warps
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(kDq4Ctas, static_cast<unsigned>(p.group));
-  cfg.blockDim = dim3(128);
+  cfg.gridDim = dim3(static_cast<unsigned>(pairs), share ? static_cast<unsigned>(p.group) : 1u);
+  cfg.blockDim = dim3(share ? kDq4JoinWarps * 32 : 32 * std::min(p.group, 8));
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D>, p) == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+  const cudaError_t e = share ? cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D, true>, p)
+                              : cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D, false>, p);
+  return e == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }
 
 int validate_decode_q4(const hcp_decode_q4_args* a) {
@@ -969,7 +987,7 @@ int validate_decode_q4(const hcp_decode_q4_args* a) {
   if (a->out_dtype != a->dtype && a->out_dtype != HCP_F32) return HCP_ERR_UNSUPPORTED;
   if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return HCP_ERR_INVALID;
   if (a->q_rows < 0) return HCP_ERR_INVALID;
-  if (a->q_rows > INT32_MAX / 2) return HCP_ERR_UNSUPPORTED;
+  if (a->q_rows > INT32_MAX / 2 / Hkv) return HCP_ERR_UNSUPPORTED;
   if (a->q_rows == 0) return HCP_OK;
   const int64_t row = static_cast<int64_t>(H) * D;
   if (a->q == nullptr || a->out == nullptr || a->kv_lens == nullptr || a->q_row_stride < row || a->out_row_stride < row ||
@@ -980,14 +998,18 @@ int validate_decode_q4(const hcp_decode_q4_args* a) {
       a->block_table_stride < a->block_table_width)
     return HCP_ERR_INVALID;
   if (a->block_table_width > INT32_MAX / a->block_size - 1) return HCP_ERR_UNSUPPORTED;
+  // tiles of the cache, and of a row with all its heads, are counted in 32 bits
+  if (a->num_blocks * (a->block_size / kQ4TileTokens) > INT32_MAX / Hkv ||
+      a->block_table_width * (a->block_size / kQ4TileTokens) > INT32_MAX / Hkv)
+    return HCP_ERR_UNSUPPORTED;
   if (a->token_req == nullptr && a->block_table_rows < a->q_rows) return HCP_ERR_INVALID;
   if (a->lse != nullptr && a->lse_stride < a->q_rows) return HCP_ERR_INVALID;
   return HCP_OK;
 }
 
 // Workspace: descriptors, then (base, sum) pairs, then partial sums, each 16-byte aligned.
-int64_t dq4_desc_bytes() { return static_cast<int64_t>(kDq4Ctas) * 16; }
-int64_t dq4_ml_bytes(int group) { return static_cast<int64_t>(kDq4Ctas) * 2 * group * 8; }
+int64_t dq4_desc_bytes(int64_t rows, int hkv) { return rows * hkv * 16; }
+int64_t dq4_ml_bytes(int group) { return static_cast<int64_t>(kDq4MaxPieces) * 2 * group * 8; }
 
 }  // namespace
 
@@ -1152,7 +1174,8 @@ extern "C" int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, 
 extern "C" int64_t hcp_decode_q4_workspace_bytes(const hcp_decode_q4_args* a) {
   if (validate_decode_q4(a) != HCP_OK) return -1;
   const int G = a->num_heads / a->num_kv_heads;
-  return dq4_desc_bytes() + dq4_ml_bytes(G) + static_cast<int64_t>(kDq4Ctas) * 2 * G * a->head_dim * 4;
+  return dq4_desc_bytes(a->q_rows, a->num_kv_heads) + dq4_ml_bytes(G) +
+         static_cast<int64_t>(kDq4MaxPieces) * 2 * G * a->head_dim * 4;
 }
 
 extern "C" int hcp_decode_q4_splitkv(const hcp_decode_q4_args* a, void* stream) {
@@ -1180,8 +1203,9 @@ extern "C" int hcp_decode_q4_splitkv(const hcp_decode_q4_args* a, void* stream) 
   p.lse_stride = a->lse_stride;
   char* ws = static_cast<char*>(a->workspace);
   p.desc = reinterpret_cast<int4*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + dq4_desc_bytes());
-  p.part_o = reinterpret_cast<float*>(ws + dq4_desc_bytes() + dq4_ml_bytes(G));
+  const int64_t desc_bytes = dq4_desc_bytes(a->q_rows, a->num_kv_heads);
+  p.part_ml = reinterpret_cast<float2*>(ws + desc_bytes);
+  p.part_o = reinterpret_cast<float*>(ws + desc_bytes + dq4_ml_bytes(G));
   p.rows = static_cast<int>(a->q_rows);
   p.num_heads = a->num_heads;
   p.num_kv_heads = a->num_kv_heads;
@@ -1190,6 +1214,7 @@ extern "C" int hcp_decode_q4_splitkv(const hcp_decode_q4_args* a, void* stream) 
   p.sub_shift = pow2_shift(a->block_size / kQ4TileTokens);
   p.scale_log2 = a->scale * 1.4426950408889634f;
   p.out_dt = a->out_dtype;
+  p.out_vec = aligned16(a->out) && a->out_row_stride % (a->out_dtype == HCP_F32 ? 4 : 8) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool f16 = a->dtype == HCP_F16, wide = G > 8;
   if (a->head_dim == 128) {
