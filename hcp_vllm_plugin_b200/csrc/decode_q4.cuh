@@ -7,11 +7,13 @@
 //
 // Bound by HBM: 9/8 D bytes per key and KV head (K and V), against 2 G D
 // products.  What has to be kept small is the work per byte.  So:
-//   * the whole numbers n - 8 are the matrix operands, exact in fp16; scales and
-//     lowest values are applied outside in 32 bits, per 64-dim group:
-//       q . k  = sum_g  s_g (q_g . (n_g - 8)) + (lo_g + 8 s_g) sum(q_g)
-//       o_g    = sum_j (p_j s_j) (n_j - 8)    + sum_j p_j (lo_j + 8 s_j)
-//     (centred, the accumulated sums stay as small as the result's own terms);
+//   * the whole numbers n are the matrix operands, exact in fp16; scales and lowest
+//     values are applied outside in 32 bits, per 64-dim group:
+//       q . k  = sum_g  s_g (q_g . (64 + n_g)) + (lo_g - 64 s_g) sum(q_g)
+//       o_g    = sum_j (p_j s_j) (n_j - 8)     + sum_j p_j (lo_j + 8 s_j)
+//     V is centred, so that sums over many keys stay as small as their own terms; a
+//     score's sum is over 64 products, where the offset costs 6 bits of 24 and saves
+//     the centring (a seventh of the kernel's instructions);
 //   * keys are the rows of the first product (16 keys x 8 heads) and dims those of
 //     the second (16 dims x 8 heads), so a group of up to 8 query heads fills the
 //     instruction's 8 columns instead of half of 16 rows;
@@ -131,6 +133,16 @@ __device__ __forceinline__ void q4_pairs(uint32_t w, const Q4Consts& c, uint32_t
   }
 }
 
+// The same pairs as 1024 + 16 n, without the centring: for products whose sums start
+// anew in every tile, where 16 (64 + n) costs 6 bits of 24 and the offset's share is
+// known (64 times the sum of the other operand).
+__device__ __forceinline__ void q4_pairs_raw(uint32_t w, const Q4Consts& c, uint32_t (&r)[4]) {
+  const uint32_t v[4] = {w << 4, w, w >> 4, w >> 8};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(r[i]) : "r"(v[i]), "r"(c.k1024));
+}
+
 // Tiles of a row (0 for a padding row or an empty one).
 __device__ __forceinline__ int dq4_len(const DecodeQ4Params& p, int r, int& req) {
   req = p.token_req != nullptr ? p.token_req[r] : r;
@@ -145,8 +157,9 @@ struct Dq4Smem {
   static constexpr int kStepBytes = kDq4Step * Q4<D>::kTileBytes;
   static constexpr int kRing = kDq4Stages * kStepBytes;
   alignas(16) uint8_t ring[kDq4Warps][kRing];
-  long long start[kDq4Threads + 1];  // tiles (of one head) before each thread's run of rows
   long long wsum[kDq4Warps];
+  long long first_cum[kDq4Warps];  // tiles of the line before the row of each warp's first tile
+  int4 first[kDq4Warps];           // that row, its request, its keys
 };
 
 __device__ __forceinline__ void dq4_store(const DecodeQ4Params& p, long long row, int head, int D, int d, float v) {
@@ -191,9 +204,10 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
   // ---- the line of tiles: sums of every thread's run of rows
   const int run = (p.rows + kDq4Threads - 1) / kDq4Threads;
   long long mine = 0;
+  int last_len = 0, last_req = 0;  // of the run's last row: its only one where there are few
   for (int r = tid * run; r < min(p.rows, (tid + 1) * run); ++r) {
-    int req;
-    mine += dq4_tiles(dq4_len(p, r, req));
+    last_len = dq4_len(p, r, last_req);
+    mine += dq4_tiles(last_len);
   }
   long long inc = mine;
 #pragma unroll
@@ -203,41 +217,44 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
   }
   if (lane == 31) sm.wsum[warp] = inc;
   __syncthreads();
-  long long before = 0;
-  for (int w = 0; w < warp; ++w) before += sm.wsum[w];
-  sm.start[tid] = before + inc - mine;
-  if (tid == kDq4Threads - 1) sm.start[kDq4Threads] = before + inc;
-  // rows without keys: zeros, lse -inf, nothing to join
-  for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
-    int req;
-    const int n = dq4_len(p, r, req);
-    if (n > 0) continue;
-    if (n == 0) {
-      for (int e = tid; e < p.num_heads * D; e += kDq4Threads) dq4_store(p, r, e / D, D, e % D, 0.f);
-      if (p.lse != nullptr)
-        for (int h = tid; h < p.num_heads; h += kDq4Threads) p.lse[h * p.lse_stride + r] = -INFINITY;
-    }
-    for (int h = tid; h < Hkv; h += kDq4Threads) p.desc[static_cast<long long>(r) * Hkv + h] = make_int4(0, 0, 0, 0);
+  long long before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kDq4Warps; ++w) {
+    before += w < warp ? sm.wsum[w] : 0;
+    all += sm.wsum[w];
   }
-  __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // ---- this warp's piece of the line
-  const long long total = sm.start[kDq4Threads] * Hkv;
-  const long long pieces = static_cast<long long>(gridDim.x) * kDq4Warps;
-  const long long piece = max(1ll, (total + pieces * U - 1) / (pieces * U)) * U;
+  // ---- the warps' pieces of the line; the thread whose rows hold a piece's first tile says where
+  constexpr int kPieces = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps;
+  const long long total = all * Hkv;
+  const long long piece = max(1ll, (total + kPieces * U - 1) / (kPieces * U)) * U;
+#pragma unroll
+  for (int w = 0; w < kDq4Warps; ++w) {
+    const long long at = (static_cast<long long>(blockIdx.x) * kDq4Warps + w) * piece;
+    long long cum = (before + inc - mine) * Hkv;
+    if (at >= cum && at < cum + mine * Hkv) {
+      int r = tid * run, req = last_req, n = run == 1 ? last_len : dq4_len(p, r, req);
+      while (r + 1 < p.rows && at >= cum + static_cast<long long>(dq4_tiles(n)) * Hkv) {
+        cum += static_cast<long long>(dq4_tiles(n)) * Hkv;
+        n = dq4_len(p, ++r, req);
+      }
+      sm.first[w] = make_int4(r, req, n, 0);
+      sm.first_cum[w] = cum;
+    }
+  }
+  __syncthreads();
   const int me = blockIdx.x * kDq4Warps + warp;
   const long long f_begin = me * piece, f_end = min(total, f_begin + piece);
-  if (f_begin >= f_end) return;
-  long long f = f_begin;
-  int lo = 0, hi = kDq4Threads - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (sm.start[mid] * Hkv <= f) lo = mid; else hi = mid - 1;
+  long long f = f_begin, cum = 0;
+  int row = 0, req = 0, len = 0;
+  if (f < f_end) {
+    const int4 first = sm.first[warp];
+    row = first.x;
+    req = first.y;
+    len = first.z;
+    cum = sm.first_cum[warp];
   }
-  int row = lo * run, req;
-  long long cum = sm.start[lo] * Hkv;
-  int len = dq4_len(p, row, req);
   const uint32_t ring = ptx::smem_u32(sm.ring[warp]) + 16 * lane;
   const int sub_mask = (1 << p.sub_shift) - 1;
 
@@ -260,9 +277,20 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     auto pages = [&](int b) {
       int v = -1;
       if (32 * b + lane < n) v = __ldg(bt + ((t0 + 32 * b + lane) >> p.sub_shift));
-      return v < p.num_blocks ? v : -1;
+      return v;  // looked at when it is used
     };
     int page = pages(0), page_next = pages(1);
+    uint4 raw[NT][KW];  // q, on its way while the ring fills
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        raw[nt][w] = make_uint4(0u, 0u, 0u, 0u);
+        if (nt * 8 + g < G)
+          raw[nt][w] = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.q) + row * p.q_row_stride +
+                                                       static_cast<long long>(kvh * G + nt * 8 + g) * D + 64 * (w >> 1) +
+                                                       16 * t + 8 * (w & 1));
+      }
     uint32_t held = 0;          // bits 2k, 2k + 1: whether the tiles of the step issued k before the last are there
     int in_at = 0, out_at = 0;  // ring offsets of the next copy and of the next step to read
     auto issue = [&](int st) {
@@ -276,10 +304,12 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
         uint32_t bytes[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          const int blk = __shfl_sync(0xffffffffu, page, (U * st + u) & 31);  // -1 past the last tile too
-          there |= blk >= 0 ? 1u << u : 0u;
-          bytes[u] = blk >= 0 ? 16u : 0u;
-          const uint32_t at = (static_cast<uint32_t>(max(blk, 0) * Hkv + kvh) << p.sub_shift) + ((t0 + U * st + u) & sub_mask);
+          uint32_t blk = static_cast<uint32_t>(__shfl_sync(0xffffffffu, page, (U * st + u) & 31));  // -1 past the last tile too
+          const bool in = blk < static_cast<uint32_t>(p.num_blocks);
+          there |= in ? 1u << u : 0u;
+          bytes[u] = in ? 16u : 0u;
+          blk = in ? blk : 0u;
+          const uint32_t at = ((blk * Hkv + kvh) << p.sub_shift) + ((t0 + U * st + u) & sub_mask);
           src[u] = p.cache + 16 * lane + static_cast<uint64_t>(at) * L::kTileBytes;
         }
         constexpr int kChunks = L::kTileBytes / 16;
@@ -302,21 +332,15 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     // scaled by a power of two to the top of fp16's range and rounded to it: exact down to
     // 2^-29 of its largest element for 11-bit elements.  The power goes into the head's factor.
     uint32_t qb[NT][2 * KW][2];
-    float sq[NT][NG][2];  // sums of the scaled q over each group, heads 2t and 2t+1
-    float hs[NT][2];      // score = hs * (scaled q . k), in log2 units
+    float sq[NT][NG][2];  // 16 times the sums of the scaled q over each group, heads 2t and 2t+1
+    float hs[NT][2];      // score in log2 units = hs * 16 (scaled q . k)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int hc = nt * 8 + g;
-      const uint16_t* qh = static_cast<const uint16_t*>(p.q) + row * p.q_row_stride +
-                           static_cast<long long>(kvh * G + hc) * D;
-      uint4 raw[KW];
       float top = 0.f;
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        raw[w] = make_uint4(0u, 0u, 0u, 0u);
-        if (hc < G) raw[w] = *reinterpret_cast<const uint4*>(qh + 64 * (w >> 1) + 16 * t + 8 * (w & 1));
         float x[8];
-        q4_unpack8<F16>(raw[w], x);
+        q4_unpack8<F16>(raw[nt][w], x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
       }
@@ -332,7 +356,7 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         float x[8];
-        q4_unpack8<F16>(raw[w], x);
+        q4_unpack8<F16>(raw[nt][w], x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           x[i] *= up;
@@ -347,10 +371,10 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
       for (int a = 0; a < NG; ++a) {
         part[a] += __shfl_xor_sync(0xffffffffu, part[a], 1);
         part[a] += __shfl_xor_sync(0xffffffffu, part[a], 2);
-        sq[nt][a][0] = __shfl_sync(0xffffffffu, part[a], 8 * t);
-        sq[nt][a][1] = __shfl_sync(0xffffffffu, part[a], 8 * t + 4);
+        sq[nt][a][0] = 16.f * __shfl_sync(0xffffffffu, part[a], 8 * t);
+        sq[nt][a][1] = 16.f * __shfl_sync(0xffffffffu, part[a], 8 * t + 4);
       }
-      const float down = p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      const float down = 0.0625f * p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
       hs[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
       hs[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
     }
@@ -423,8 +447,8 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             uint32_t x[4], y[4];
-            q4_pairs(kw[0][2 * a + e], consts, x);
-            q4_pairs(kw[1][2 * a + e], consts, y);
+            q4_pairs_raw(kw[0][2 * a + e], consts, x);
+            q4_pairs_raw(kw[1][2 * a + e], consts, y);
             const uint32_t fa[4] = {x[0], y[0], x[1], y[1]}, fb[4] = {x[2], y[2], x[3], y[3]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -434,14 +458,18 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
               mma16816<true>(acc[nt], fb, qb[nt][kk + 1][0], qb[nt][kk + 1][1]);
             }
           }
-          const float s0 = q4_up<F16>(prm[u][0][a] & 0xffffu), z0 = fmaf(8.f, s0, q4_up<F16>(prm[u][0][a] >> 16));
-          const float s1 = q4_up<F16>(prm[u][1][a] & 0xffffu), z1 = fmaf(8.f, s1, q4_up<F16>(prm[u][1][a] >> 16));
+          const float s0 = q4_up<F16>(prm[u][0][a] & 0xffffu), z0 = fmaf(-64.f, s0, q4_up<F16>(prm[u][0][a] >> 16));
+          const float s1 = q4_up<F16>(prm[u][1][a] & 0xffffu), z1 = fmaf(-64.f, s1, q4_up<F16>(prm[u][1][a] >> 16));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float zq = a == 0 ? (e < 2 ? z0 : z1) * sq[nt][a][e & 1] : fmaf(e < 2 ? z0 : z1, sq[nt][a][e & 1], sc[u][nt][e]);
-              sc[u][nt][e] = fmaf(e < 2 ? s0 : s1, acc[nt][e], zq);
+            for (int e = 0; e < 2; ++e) {
+              const float2 zz = make_float2(e == 0 ? z0 : z1, e == 0 ? z0 : z1), ss = make_float2(e == 0 ? s0 : s1, e == 0 ? s0 : s1);
+              const float2 qq = make_float2(sq[nt][a][0], sq[nt][a][1]);
+              const float2 zq = a == 0 ? __fmul2_rn(zz, qq) : __ffma2_rn(zz, qq, make_float2(sc[u][nt][2 * e], sc[u][nt][2 * e + 1]));
+              const float2 r = __ffma2_rn(ss, make_float2(acc[nt][2 * e], acc[nt][2 * e + 1]), zq);
+              sc[u][nt][2 * e] = r.x;
+              sc[u][nt][2 * e + 1] = r.y;
             }
         }
         if (!whole_step) {
@@ -532,10 +560,18 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) pr[u][nt][e] = ex2_approx(fmaf(sc[u][nt][e], hs[nt][e & 1], -base[nt][e & 1]));
-          l_run[nt][0] += pr[u][nt][0] + pr[u][nt][2];
-          l_run[nt][1] += pr[u][nt][1] + pr[u][nt][3];
+          // pairs of heads in packed arithmetic
+          const float2 f = make_float2(hs[nt][0], hs[nt][1]), b = make_float2(-base[nt][0], -base[nt][1]);
+          const float2 x0 = __ffma2_rn(make_float2(sc[u][nt][0], sc[u][nt][1]), f, b);
+          const float2 x1 = __ffma2_rn(make_float2(sc[u][nt][2], sc[u][nt][3]), f, b);
+          pr[u][nt][0] = ex2_approx(x0.x);
+          pr[u][nt][1] = ex2_approx(x0.y);
+          pr[u][nt][2] = ex2_approx(x1.x);
+          pr[u][nt][3] = ex2_approx(x1.y);
+          const float2 l = __fadd2_rn(make_float2(l_run[nt][0], l_run[nt][1]),
+                                      __fadd2_rn(make_float2(pr[u][nt][0], pr[u][nt][1]), make_float2(pr[u][nt][2], pr[u][nt][3])));
+          l_run[nt][0] = l.x;
+          l_run[nt][1] = l.y;
         }
       // ---- O += V^T P per group
 #pragma unroll
@@ -550,10 +586,13 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
           uint32_t bp[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            vz[nt][a][0] = fmaf(pr[u][nt][0], z0, fmaf(pr[u][nt][2], z1, vz[nt][a][0]));
-            vz[nt][a][1] = fmaf(pr[u][nt][1], z0, fmaf(pr[u][nt][3], z1, vz[nt][a][1]));
-            bp[nt][0] = movmatrix_t(pack2<true>(pr[u][nt][0] * s0, pr[u][nt][1] * s0));
-            bp[nt][1] = movmatrix_t(pack2<true>(pr[u][nt][2] * s1, pr[u][nt][3] * s1));
+            const float2 p0 = make_float2(pr[u][nt][0], pr[u][nt][1]), p1 = make_float2(pr[u][nt][2], pr[u][nt][3]);
+            const float2 zv = __ffma2_rn(p0, make_float2(z0, z0), __ffma2_rn(p1, make_float2(z1, z1), make_float2(vz[nt][a][0], vz[nt][a][1])));
+            vz[nt][a][0] = zv.x;
+            vz[nt][a][1] = zv.y;
+            const float2 y0 = __fmul2_rn(p0, make_float2(s0, s0)), y1 = __fmul2_rn(p1, make_float2(s1, s1));
+            bp[nt][0] = movmatrix_t(pack2<true>(y0.x, y0.y));
+            bp[nt][1] = movmatrix_t(pack2<true>(y1.x, y1.y));
           }
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
@@ -572,37 +611,41 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     const int slot = f == f_begin ? 0 : 1;
     const long long part = (static_cast<long long>(me) * 2 + slot) * G;
 #pragma unroll
+    for (int s = 4; s < 32; s <<= 1)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          l_run[nt][e] += __shfl_xor_sync(0xffffffffu, l_run[nt][e], s);
+#pragma unroll
+          for (int a = 0; a < NG; ++a) vz[nt][a][e] += __shfl_xor_sync(0xffffffffu, vz[nt][a][e], s);
+        }
+#pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float l = l_run[nt][e];
-#pragma unroll
-        for (int s = 4; s < 32; s <<= 1) l += __shfl_xor_sync(0xffffffffu, l, s);
+        const float l = l_run[nt][e];
         const int h = nt * 8 + 2 * t + e;
-        const float inv = whole ? (l == 0.f ? 0.f : 1.f / l) : 1.f;
+        if (h >= G) continue;
+        const float inv = whole ? (l == 0.f ? 0.f : __fdividef(1.f, l)) : 1.f;
 #pragma unroll
         for (int a = 0; a < NG; ++a) {
-          float z = vz[nt][a][e];
-#pragma unroll
-          for (int s = 4; s < 32; s <<= 1) z += __shfl_xor_sync(0xffffffffu, z, s);
           float v[8];
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
-            v[2 * i2] = fmaf(o[nt][a][i2][e], vref[a], z) * inv;
-            v[2 * i2 + 1] = fmaf(o[nt][a][i2][e + 2], vref[a], z) * inv;
+            v[2 * i2] = fmaf(o[nt][a][i2][e], vref[a], vz[nt][a][e]) * inv;
+            v[2 * i2 + 1] = fmaf(o[nt][a][i2][e + 2], vref[a], vz[nt][a][e]) * inv;
           }
           const int d = 8 * (8 * a + g);
-          if (h < G) {
-            if (whole) {
-              dq4_store8(p, row, kvh * G + h, D, d, v);
-            } else {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + (part + h) * D + d);
-              dst[0] = make_float4(v[0], v[1], v[2], v[3]);
-              dst[1] = make_float4(v[4], v[5], v[6], v[7]);
-            }
+          if (whole) {
+            dq4_store8(p, row, kvh * G + h, D, d, v);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + (part + h) * D + d);
+            dst[0] = make_float4(v[0], v[1], v[2], v[3]);
+            dst[1] = make_float4(v[4], v[5], v[6], v[7]);
           }
         }
-        if (g == 0 && h < G) {
+        if (g == 0) {
           if (!whole) {
             // no key yet: base -inf, but a NaN sum must show
             p.part_ml[part + h] = make_float2(l == 0.f ? -INFINITY : base[nt][e], l);
@@ -612,10 +655,26 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
         }
       }
     if (t0 == 0 && lane == 0) {
-      const long long last = (f + tiles - 1) / piece;
-      p.desc[static_cast<long long>(row) * Hkv + kvh] = make_int4(me, slot, whole ? 0 : static_cast<int>(last - me) + 1, 0);
+      int parts = 0;
+      if (!whole) {
+        const long long end = f - f_begin + tiles - 1;  // its last tile, from this piece's first
+        parts = 1 + static_cast<int>(end <= INT_MAX && piece <= INT_MAX ? static_cast<uint32_t>(end) / static_cast<uint32_t>(piece)
+                                                                         : end / piece);
+      }
+      p.desc[static_cast<long long>(row) * Hkv + kvh] = make_int4(me, slot, parts, 0);
     }
     f += n;
+  }
+  // ---- rows without keys (zeros, lse -inf) and padding rows have nothing to join; the last warps have least to do
+  for (int r = kPieces - 1 - me; r < p.rows; r += kPieces) {
+    const int n = dq4_len(p, r, req);
+    if (n > 0) continue;
+    if (n == 0) {
+      for (int e = lane; e < p.num_heads * D; e += 32) dq4_store(p, r, e / D, D, e % D, 0.f);
+      if (p.lse != nullptr)
+        for (int h = lane; h < p.num_heads; h += 32) p.lse[h * p.lse_stride + r] = -INFINITY;
+    }
+    for (int h = lane; h < Hkv; h += 32) p.desc[static_cast<long long>(r) * Hkv + h] = make_int4(0, 0, 0, 0);
   }
 }
 
@@ -627,7 +686,7 @@ __global__ void __launch_bounds__(kDq4JoinWarps * 32, 2) decode_q4_join_kernel(c
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 desc = p.desc[blockIdx.x];
   if (desc.z <= 0 || desc.x < 0 || desc.x + desc.z > kDq4MaxPieces || (desc.y & ~1) != 0) return;
-  constexpr int V = D / 32;
+  constexpr int V = D / 32;  // neighbouring dims of a lane
   const int G = p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int row = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
   __shared__ float so[SHARE ? kDq4JoinWarps : 1][D], sl[kDq4JoinWarps], smx[kDq4JoinWarps];
@@ -647,20 +706,30 @@ __global__ void __launch_bounds__(kDq4JoinWarps * 32, 2) decode_q4_join_kernel(c
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.f;
     if (M != -INFINITY) {
-#pragma unroll 4
+#pragma unroll 8
       for (int i = SHARE ? warp : 0; i < desc.z; i += SHARE ? warps : 1) {
         const long long at = index(i);
         const float2 ml = p.part_ml[at];
         const float x = ex2_approx(ml.x - M);
         ls = fmaf(x, ml.y, ls);
-#pragma unroll
-        for (int v = 0; v < V; ++v) acc[v] = fmaf(x, p.part_o[at * D + v * 32 + lane], acc[v]);
+        const float* part = p.part_o + at * D + V * lane;
+        if constexpr (V == 4) {
+          const float4 o = *reinterpret_cast<const float4*>(part);
+          acc[0] = fmaf(x, o.x, acc[0]);
+          acc[1] = fmaf(x, o.y, acc[1]);
+          acc[2] = fmaf(x, o.z, acc[2]);
+          acc[3] = fmaf(x, o.w, acc[3]);
+        } else {
+          const float2 o = *reinterpret_cast<const float2*>(part);
+          acc[0] = fmaf(x, o.x, acc[0]);
+          acc[1] = fmaf(x, o.y, acc[1]);
+        }
       }
     }
     const int head = kvh * G + h;
     if constexpr (SHARE) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) so[warp][v * 32 + lane] = acc[v];
+      for (int v = 0; v < V; ++v) so[warp][V * lane + v] = acc[v];
       if (lane == 0) sl[warp] = ls;
       __syncthreads();
       ls = 0.f;
@@ -673,7 +742,7 @@ __global__ void __launch_bounds__(kDq4JoinWarps * 32, 2) decode_q4_join_kernel(c
       __syncthreads();
     } else {
 #pragma unroll
-      for (int v = 0; v < V; ++v) dq4_store(p, row, head, D, v * 32 + lane, ls == 0.f ? 0.f : acc[v] / ls);
+      for (int v = 0; v < V; ++v) dq4_store(p, row, head, D, V * lane + v, ls == 0.f ? 0.f : acc[v] / ls);
     }
     if ((SHARE ? threadIdx.x : lane) == 0 && p.lse != nullptr)
       p.lse[head * p.lse_stride + row] = ls == 0.f ? -INFINITY : (M + lg2_approx(ls)) * 0.69314718055994530942f;

@@ -966,7 +966,10 @@ int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
   const bool share = pairs <= kDq4Sms;  // one pair or a few an SM: their parts are shared between warps
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(pairs), share ? static_cast<unsigned>(p.group) : 1u);
-  cfg.blockDim = dim3(share ? kDq4JoinWarps * 32 : 32 * std::min(p.group, 8));
+  // parts of a pair, were the rows alike: 8 a warp, which loads them at once
+  const int64_t parts = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps / pairs + 2;
+  const int warps = share ? static_cast<int>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8)) : std::min(p.group, 8);
+  cfg.blockDim = dim3(32 * warps);
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
