@@ -927,18 +927,27 @@ namespace {
 bool q4_block_size(int bs) { return bs == 16 || bs == 32 || bs == 64 || bs == 128; }
 bool aligned8(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 7u) == 0; }
 
+// Runs of 16 tokens; one more, as the first may begin inside a tile.
+int64_t q4_runs(int64_t tokens) { return (tokens + kQ4TileTokens - 1) / kQ4TileTokens + 1; }
+
 template <int D, bool F16, bool TAB32>
-int launch_norm_rope(const NormRopeParams& p, int64_t tokens, int kind, cudaStream_t st) {
+int launch_norm_rope(NormRopeParams p, int64_t tokens, int kind, cudaStream_t st) {
   constexpr int per_round = kRopeThreads / (D / 8);
-  const int rows = p.num_heads + p.num_kv_heads * (kind == HCP_ROPE_CACHE_NONE ? 1 : 2);
+  const int rows = p.num_heads + (kind == HCP_ROPE_CACHE_Q4 ? 0 : p.num_kv_heads);
   const int rounds = (rows + per_round - 1) / per_round;
   // few tokens: one round a block, so the whole token is in flight at once
-  const int spread = tokens * rounds <= 8 * 148 ? rounds : 1;
-  const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(spread));
+  p.spread = tokens * rounds <= 8 * 148 ? rounds : 1;
+  p.num_tokens = tokens;
+  int64_t grid = tokens * p.spread;
+  const int64_t kv_blocks = kind == HCP_ROPE_CACHE_Q4 ? q4_runs(tokens) * p.num_kv_heads : 0;
+  grid += kv_blocks;
+  if (grid > INT32_MAX) return HCP_ERR_UNSUPPORTED;
+  p.kv_blocks = static_cast<unsigned>(kv_blocks);
+  const unsigned blocks = static_cast<unsigned>(grid);
   switch (kind) {
-    case HCP_ROPE_CACHE_SAME: norm_rope_kernel<D, F16, TAB32, kRopeCacheSame><<<grid, kRopeThreads, 0, st>>>(p); break;
-    case HCP_ROPE_CACHE_Q4: norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4><<<grid, kRopeThreads, 0, st>>>(p); break;
-    default: norm_rope_kernel<D, F16, TAB32, kRopeCacheNone><<<grid, kRopeThreads, 0, st>>>(p); break;
+    case HCP_ROPE_CACHE_SAME: norm_rope_kernel<D, F16, TAB32, kRopeCacheSame><<<blocks, kRopeThreads, 0, st>>>(p); break;
+    case HCP_ROPE_CACHE_Q4: norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4><<<blocks, kRopeThreads, 0, st>>>(p); break;
+    default: norm_rope_kernel<D, F16, TAB32, kRopeCacheNone><<<blocks, kRopeThreads, 0, st>>>(p); break;
   }
   return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }
@@ -1128,15 +1137,16 @@ extern "C" int hcp_kv_cache_update_q4(const void* key, const void* value, int64_
   p.block_size = block_size;
   p.bs_shift = pow2_shift(block_size);
   p.num_kv_heads = num_kv_heads;
-  const int per_block = 256 / (head_dim / 4);
-  const dim3 grid(static_cast<unsigned>((num_tokens + per_block - 1) / per_block), static_cast<unsigned>(num_kv_heads));
+  const int64_t units = q4_runs(num_tokens) * num_kv_heads;
+  if (units > INT32_MAX) return HCP_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(units);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128) {
-    if (dtype == HCP_F16) q4_update_kernel<128, true><<<grid, 256, 0, st>>>(p);
-    else q4_update_kernel<128, false><<<grid, 256, 0, st>>>(p);
+    if (dtype == HCP_F16) q4_update_kernel<128, true><<<grid, kQ4Threads, 0, st>>>(p);
+    else q4_update_kernel<128, false><<<grid, kQ4Threads, 0, st>>>(p);
   } else {
-    if (dtype == HCP_F16) q4_update_kernel<64, true><<<grid, 256, 0, st>>>(p);
-    else q4_update_kernel<64, false><<<grid, 256, 0, st>>>(p);
+    if (dtype == HCP_F16) q4_update_kernel<64, true><<<grid, kQ4Threads, 0, st>>>(p);
+    else q4_update_kernel<64, false><<<grid, kQ4Threads, 0, st>>>(p);
   }
   return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }
@@ -1161,15 +1171,16 @@ extern "C" int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, 
   p.block_size = block_size;
   p.bs_shift = pow2_shift(block_size);
   p.num_kv_heads = num_kv_heads;
-  const int per_block = 256 / (head_dim / 4);
-  const dim3 grid(static_cast<unsigned>((num_tokens + per_block - 1) / per_block), static_cast<unsigned>(num_kv_heads));
+  const int64_t blocks = (q4_runs(num_tokens) * num_kv_heads + kQ4Threads / 32 - 1) / (kQ4Threads / 32);
+  if (blocks > INT32_MAX) return HCP_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (head_dim == 128) {
-    if (dtype == HCP_F16) q4_gather_kernel<128, true><<<grid, 256, 0, st>>>(p);
-    else q4_gather_kernel<128, false><<<grid, 256, 0, st>>>(p);
+    if (dtype == HCP_F16) q4_gather_kernel<128, true><<<grid, kQ4Threads, 0, st>>>(p);
+    else q4_gather_kernel<128, false><<<grid, kQ4Threads, 0, st>>>(p);
   } else {
-    if (dtype == HCP_F16) q4_gather_kernel<64, true><<<grid, 256, 0, st>>>(p);
-    else q4_gather_kernel<64, false><<<grid, 256, 0, st>>>(p);
+    if (dtype == HCP_F16) q4_gather_kernel<64, true><<<grid, kQ4Threads, 0, st>>>(p);
+    else q4_gather_kernel<64, false><<<grid, kQ4Threads, 0, st>>>(p);
   }
   return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }

@@ -11,9 +11,10 @@
 // Bound by HBM: 2 bytes read and 2 written per element.  D/8 lanes own a row and
 // each lane holds both members of its pairs (4 dims and their 4 partners), so the
 // rotation needs no exchange.  A block works on one token: its lanes load the
-// weights and the token's cos / sin once and go over the token's heads, all loads
-// of a round in flight before the first is used.  With few tokens the heads are
-// spread over blocks instead (gridDim.y), one round each.
+// token's cos / sin once and go over the token's heads, two rows' loads in flight.
+// With few tokens the heads are spread over blocks instead, one round each.  With the
+// 4-bit cache further blocks of the same launch take k and v, 16 tokens of one head
+// each, so that whole tiles of the cache are built in shared memory (q4_cache.cuh).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -50,6 +51,9 @@ struct NormRopeParams {
   int interleaved;
   int block_size;
   int bs_shift;
+  long long num_tokens;
+  int spread;                  // blocks of a token
+  unsigned kv_blocks;          // blocks that take k and v, with the 4-bit cache
 };
 
 template <bool F16>
@@ -64,183 +68,241 @@ __device__ __forceinline__ uint2 rope_down4(const float* x) {
   return make_uint2(q4_down<F16>(x[0]) | (q4_down<F16>(x[1]) << 16), q4_down<F16>(x[2]) | (q4_down<F16>(x[3]) << 16));
 }
 
-// 4 dims starting at d (a multiple of 4) of a token's K row.
-template <int D>
-__device__ __forceinline__ void q4_store_k4(uint8_t* tile, int j, int d, const float* x, float s, float m) {
-  uint32_t w = 0;
+// This lane's dims of a row: a0 .. a0+3 and a1 .. a1+3, partners where it turns them.
+struct RopeLane {
+  int a0, a1;
+  bool turns;
+};
+__device__ __forceinline__ RopeLane rope_lane(const NormRopeParams& p, int c) {
+  RopeLane r;
+  const int pairs = p.rotary / 8;  // lanes that rotate
+  r.turns = c < pairs;
+  r.a0 = !r.turns ? p.rotary + 8 * (c - pairs) : p.interleaved ? 8 * c : 4 * c;
+  r.a1 = r.turns && !p.interleaved ? p.rotary / 2 + 4 * c : r.a0 + 4;
+  return r;
+}
+template <bool F16, bool TAB32>
+__device__ __forceinline__ void rope_angles(const NormRopeParams& p, long long pos, int c, float* cs, float* sn) {
+  const long long at = pos * p.table_stride + 4 * c;
+  if constexpr (TAB32) {
+    const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + at);
+    const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + at + p.rotary / 2);
+    cs[0] = a.x; cs[1] = a.y; cs[2] = a.z; cs[3] = a.w;
+    sn[0] = b.x; sn[1] = b.y; sn[2] = b.z; sn[3] = b.w;
+  } else {
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.table) + at), cs);
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.table) + at + p.rotary / 2), sn);
+  }
+}
+// Norm and rotation of one row; every lane of the warp takes part.
+template <int D, bool F16>
+__device__ __forceinline__ void rope_row(const NormRopeParams& p, const RopeLane& r, const uint16_t* w, bool known,
+                                         const float* cs, const float* sn, const uint2 (&in)[2], uint2 (&out)[2]) {
+  float x[8];
+  rope_up4<F16>(in[0], x);
+  rope_up4<F16>(in[1], x + 4);
+  float sq = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w |= q4_code(x[i], s, m) << (4 * i);
-  *reinterpret_cast<uint16_t*>(tile + j * (D / 2) + Q4<D>::k_word(d >> 3) + ((d >> 2) & 1) * 2) =
-      static_cast<uint16_t>(w);
+  for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
+#pragma unroll
+  for (int s = 1; s < D / 8; s <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, s);
+  if (w != nullptr) {
+    const float inv = rsqrtf(sq * (1.f / D) + p.eps);
+    float g[8];
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a0), g);
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a1), g + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
+  }
+  float y[8];
+  if (!r.turns) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+  } else if (p.interleaved) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
+      y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      y[i] = x[i] * cs[i] - x[i + 4] * sn[i];
+      y[i + 4] = x[i + 4] * cs[i] + x[i] * sn[i];
+    }
+  }
+  if (!known) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fffffff);
+  }
+  out[0] = rope_down4<F16>(y);
+  out[1] = rope_down4<F16>(y + 4);
 }
 
+// k and v of 16 tokens of one head: k normed, rotated and written to k_out, both into the cache.
+template <int D, bool F16, bool TAB32>
+__device__ __forceinline__ void rope_kv_block(const NormRopeParams& p, int unit, Q4Stage<D>& st) {
+  using L = Q4<D>;
+  constexpr int kRows = kRopeThreads / L::kLanes;
+  const int h = unit % p.num_kv_heads;
+  long long t0;
+  long long slot = q4_run_slots(p.slot_mapping, p.num_tokens, unit / p.num_kv_heads, t0);
+  if (t0 >= p.num_tokens) return;
+  if (threadIdx.x < 32) {
+    Q4UpdateParams u;
+    u.num_blocks = p.num_blocks;
+    u.block_size = p.block_size;
+    u.bs_shift = p.bs_shift;
+    u.num_kv_heads = p.num_kv_heads;
+    if (slot >= 0) {
+      const long long pos = p.positions[t0 + threadIdx.x];
+      if (pos < 0 || pos >= p.table_rows) slot = -1;
+    }
+    q4_place<D>(st, u, slot, h);
+  }
+  const int c = threadIdx.x % L::kLanes;
+  const RopeLane ln = rope_lane(p, c);
+#pragma unroll 2
+  for (int row = threadIdx.x / L::kLanes; row < kQ4TileTokens; row += kRows) {
+    const long long tok = t0 + row;
+    const bool here = tok >= 0 && tok < p.num_tokens;
+    const long long pos = here ? p.positions[tok] : -1;
+    const bool known = pos < p.table_rows;
+    uint2 in[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)}, out[2];
+    uint4 vraw = make_uint4(0u, 0u, 0u, 0u);
+    float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
+    if (here) {
+      const uint16_t* k = p.k + tok * p.k_stride + static_cast<long long>(h) * D;
+      in[0] = *reinterpret_cast<const uint2*>(k + ln.a0);
+      in[1] = *reinterpret_cast<const uint2*>(k + ln.a1);
+      vraw = reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + static_cast<long long>(h) * D)[c];
+    }
+    if (ln.turns && known && pos >= 0) rope_angles<F16, TAB32>(p, pos, c, cs, sn);
+    rope_row<D, F16>(p, ln, p.k_weight, known, cs, sn, in, out);
+    if (pos >= 0) {
+      uint16_t* k = p.k_out + tok * p.k_out_stride + static_cast<long long>(h) * D;
+      *reinterpret_cast<uint2*>(k + ln.a0) = out[0];
+      *reinterpret_cast<uint2*>(k + ln.a1) = out[1];
+    }
+    float z[8], x[8];  // the rounded key, the value
+    rope_up4<F16>(out[0], z);
+    rope_up4<F16>(out[1], z + 4);
+    q4_unpack8<F16>(vraw, x);
+    // K: ranges of both groups over the row's lanes (a lane may hold dims of both); V: of the lane's group
+    constexpr uint32_t kInf = q4_inf2<F16>(), kNegInf = kInf | 0x80008000u;
+    uint32_t lo[L::kGroups], hi[L::kGroups];
+#pragma unroll
+    for (int g = 0; g < L::kGroups; ++g) {
+      const bool i0 = (ln.a0 >> 6) == g, i1 = (ln.a1 >> 6) == g;
+      lo[g] = q4_min2<F16>(i0 ? q4_min2<F16>(out[0].x, out[0].y) : kInf, i1 ? q4_min2<F16>(out[1].x, out[1].y) : kInf);
+      hi[g] = q4_max2<F16>(i0 ? q4_max2<F16>(out[0].x, out[0].y) : kNegInf, i1 ? q4_max2<F16>(out[1].x, out[1].y) : kNegInf);
+    }
+    uint32_t vlo = q4_min2<F16>(q4_min2<F16>(vraw.x, vraw.y), q4_min2<F16>(vraw.z, vraw.w));
+    uint32_t vhi = q4_max2<F16>(q4_max2<F16>(vraw.x, vraw.y), q4_max2<F16>(vraw.z, vraw.w));
+#pragma unroll
+    for (int s = 1; s < L::kLanes; s <<= 1) {
+#pragma unroll
+      for (int g = 0; g < L::kGroups; ++g) {
+        lo[g] = q4_min2<F16>(lo[g], __shfl_xor_sync(0xffffffffu, lo[g], s));
+        hi[g] = q4_max2<F16>(hi[g], __shfl_xor_sync(0xffffffffu, hi[g], s));
+      }
+      if (s < 8) {
+        vlo = q4_min2<F16>(vlo, __shfl_xor_sync(0xffffffffu, vlo, s));
+        vhi = q4_max2<F16>(vhi, __shfl_xor_sync(0xffffffffu, vhi, s));
+      }
+    }
+    float s[L::kGroups], m[L::kGroups], vs, vm;
+#pragma unroll
+    for (int g = 0; g < L::kGroups; ++g) q4_params<F16>(lo[g], hi[g], s[g], m[g]);
+    q4_params<F16>(vlo, vhi, vs, vm);
+    constexpr int kLast = L::kGroups - 1;
+    const bool u0 = ln.a0 < 64, u1 = ln.a1 < 64;
+    q4_stage_k4<D>(st, row, ln.a0, q4_codes<4>(z, u0 ? s[0] : s[kLast], u0 ? m[0] : m[kLast]));
+    q4_stage_k4<D>(st, row, ln.a1, q4_codes<4>(z + 4, u1 ? s[0] : s[kLast], u1 ? m[0] : m[kLast]));
+    q4_stage_v8<D>(st, row, c, q4_codes<8>(x, vs, vm));
+    if (c < L::kGroups) q4_stage_params<D, F16>(st, row, 0, c, c == 0 ? s[0] : s[kLast], c == 0 ? m[0] : m[kLast]);
+    if ((c & 7) == 0) q4_stage_params<D, F16>(st, row, 1, c >> 3, vs, vm);
+  }
+  __syncthreads();
+  q4_flush<D>(st, static_cast<uint8_t*>(p.cache));
+}
+
+// Blocks 0 .. kv_blocks - 1 (with the 4-bit cache; the longer ones come first): k and v, 16
+// tokens of one head each.  The blocks after them: rows of one token each.
 template <int D, bool F16, bool TAB32, int CACHE>
 __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeParams p) {
   constexpr int kLanes = D / 8;
   constexpr int kRows = kRopeThreads / kLanes;   // rows of a round
-  const long long tok = blockIdx.x;
-  const int c = threadIdx.x % kLanes;
   const int H = p.num_heads, Hkv = p.num_kv_heads;
-  const int rows = H + Hkv + (CACHE != kRopeCacheNone ? Hkv : 0);
+  if constexpr (CACHE == kRopeCacheQ4) {
+    __shared__ Q4Stage<D> st;
+    if (blockIdx.x < p.kv_blocks) {
+      rope_kv_block<D, F16, TAB32>(p, static_cast<int>(blockIdx.x), st);
+      return;
+    }
+  }
+  const unsigned bid = blockIdx.x - p.kv_blocks;
+  const unsigned tok32 = p.spread == 1 ? bid : bid / p.spread;
+  const int part = p.spread == 1 ? 0 : bid - tok32 * p.spread;
+  const long long tok = tok32;
+  const int c = threadIdx.x % kLanes;
+  const RopeLane ln = rope_lane(p, c);
+  const int rows = CACHE == kRopeCacheQ4 ? H : H + Hkv;
+  constexpr int U = 2;
+  uint2 in[U][2], out[2];
+  auto load = [&](int r0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * p.spread * kRows + threadIdx.x / kLanes;
+      in[u][0] = in[u][1] = make_uint2(0u, 0u);
+      if (r < rows) {
+        const uint16_t* row = r < H ? p.q + tok * p.q_stride + static_cast<long long>(r) * D
+                                    : p.k + tok * p.k_stride + static_cast<long long>(r - H) * D;
+        in[u][0] = *reinterpret_cast<const uint2*>(row + ln.a0);
+        in[u][1] = *reinterpret_cast<const uint2*>(row + ln.a1);
+      }
+    }
+  };
+  load(part * kRows);                            // beside the position
   const long long pos = p.positions[tok];
   if (pos < 0) return;                           // padding row: everything stays
   const bool known = pos < p.table_rows;
-
-  // this lane's dims: a0..a0+3 and a1..a1+3
-  const int pairs = p.rotary / 8;                // lanes that rotate
-  const bool turns = c < pairs;
-  int a0, a1;
-  if (!turns) {
-    a0 = p.rotary + 8 * (c - pairs);
-    a1 = a0 + 4;
-  } else if (p.interleaved) {
-    a0 = 8 * c;
-    a1 = a0 + 4;
-  } else {
-    a0 = 4 * c;
-    a1 = p.rotary / 2 + 4 * c;
+  float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
+  if (ln.turns && known) rope_angles<F16, TAB32>(p, pos, c, cs, sn);
+  long long dst = -1;                            // cache offset of the token's row of head 0
+  if constexpr (CACHE == kRopeCacheSame) {
+    long long blk;
+    int off;
+    if (known && slot_block(p.slot_mapping[tok], p.num_blocks, p.block_size, p.bs_shift, blk, off))
+      dst = (blk * Hkv * p.block_size + off) * 2LL * D;
   }
-  float cs[4], sn[4];
+  for (int r0 = part * kRows; r0 < rows; r0 += p.spread * kRows * U) {
+    if (r0 != part * kRows) load(r0);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    cs[i] = 1.f;
-    sn[i] = 0.f;
-  }
-  if (turns && known) {
-    const long long at = pos * p.table_stride + 4 * c;
-    if constexpr (TAB32) {
-      const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + at);
-      const float4 b = *reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + at + p.rotary / 2);
-      cs[0] = a.x; cs[1] = a.y; cs[2] = a.z; cs[3] = a.w;
-      sn[0] = b.x; sn[1] = b.y; sn[2] = b.z; sn[3] = b.w;
-    } else {
-      rope_up4<F16>(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.table) + at), cs);
-      rope_up4<F16>(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.table) + at + p.rotary / 2), sn);
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * p.spread * kRows + threadIdx.x / kLanes;
+      if (r0 + u * p.spread * kRows >= rows) break;  // the same for all
+      rope_row<D, F16>(p, ln, r < H ? p.q_weight : p.k_weight, known, cs, sn, in[u], out);
+      if (r >= rows) continue;
+      uint16_t* row = r < H ? p.q_out + tok * p.q_out_stride + static_cast<long long>(r) * D
+                            : p.k_out + tok * p.k_out_stride + static_cast<long long>(r - H) * D;
+      *reinterpret_cast<uint2*>(row + ln.a0) = out[0];
+      *reinterpret_cast<uint2*>(row + ln.a1) = out[1];
+      if constexpr (CACHE == kRopeCacheSame) {
+        if (r >= H && dst >= 0) {
+          uint16_t* to = static_cast<uint16_t*>(p.cache) + dst + static_cast<long long>(r - H) * p.block_size * 2 * D;
+          *reinterpret_cast<uint2*>(to + ln.a0) = out[0];
+          *reinterpret_cast<uint2*>(to + ln.a1) = out[1];
+        }
+      }
     }
   }
-  long long blk = 0;
-  int off = 0;
-  bool slot = false;
-  if constexpr (CACHE != kRopeCacheNone)
-    slot = known && slot_block(p.slot_mapping[tok], p.num_blocks, p.block_size, p.bs_shift, blk, off);
-
-  for (int r0 = blockIdx.y * kRows; r0 < rows; r0 += gridDim.y * kRows) {
-    const int r = r0 + threadIdx.x / kLanes;
-    const bool is_q = r < H, is_v = r >= H + Hkv, have = r < rows;
-    const int h = is_q ? r : is_v ? r - H - Hkv : r - H;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (have) {
-      if (is_v) {
-        q4_unpack8<F16>(reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + static_cast<long long>(h) * D)[c], x);
-      } else {
-        const uint16_t* row = (is_q ? p.q + tok * p.q_stride : p.k + tok * p.k_stride) + static_cast<long long>(h) * D;
-        rope_up4<F16>(*reinterpret_cast<const uint2*>(row + a0), x);
-        rope_up4<F16>(*reinterpret_cast<const uint2*>(row + a1), x + 4);
+  if constexpr (CACHE == kRopeCacheSame) {
+    if (dst >= 0)
+      for (int h = part * kRows + threadIdx.x / kLanes; h < Hkv; h += p.spread * kRows) {
+        const uint4 v = reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + static_cast<long long>(h) * D)[c];
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.cache) + dst + static_cast<long long>(h) * p.block_size * 2 * D + D)[c] = v;
       }
-    }
-    const uint16_t* w = is_q ? p.q_weight : p.k_weight;
-    float sq = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
-#pragma unroll
-    for (int s = 1; s < kLanes; s <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, s);
-    uint2 y0, y1;
-    if (!is_v) {
-      if (w != nullptr) {
-        const float inv = rsqrtf(sq * (1.f / D) + p.eps);
-        float g[8];
-        rope_up4<F16>(*reinterpret_cast<const uint2*>(w + a0), g);
-        rope_up4<F16>(*reinterpret_cast<const uint2*>(w + a1), g + 4);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-      }
-      float y[8];
-      if (!turns) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i];
-      } else if (p.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-          y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y[i] = x[i] * cs[i] - x[i + 4] * sn[i];
-          y[i + 4] = x[i + 4] * cs[i] + x[i] * sn[i];
-        }
-      }
-      if (!known)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fffffff);
-      y0 = rope_down4<F16>(y);
-      y1 = rope_down4<F16>(y + 4);
-      if (have) {
-        uint16_t* o = (is_q ? p.q_out + tok * p.q_out_stride : p.k_out + tok * p.k_out_stride) +
-                      static_cast<long long>(h) * D;
-        *reinterpret_cast<uint2*>(o + a0) = y0;
-        *reinterpret_cast<uint2*>(o + a1) = y1;
-      }
-    }
-    if constexpr (CACHE == kRopeCacheSame) {
-      if (have && slot && !is_q) {
-        uint16_t* dst = static_cast<uint16_t*>(p.cache) + ((blk * Hkv + h) * p.block_size + off) * 2LL * D;
-        if (is_v) {
-          reinterpret_cast<uint4*>(dst + D)[c] = q4_pack8<F16>(x);
-        } else {
-          *reinterpret_cast<uint2*>(dst + a0) = y0;
-          *reinterpret_cast<uint2*>(dst + a1) = y1;
-        }
-      }
-    }
-    if constexpr (CACHE == kRopeCacheQ4) {
-      // ranges of both groups over the row's lanes (every lane takes part)
-      float z[8];
-      const int d0 = is_v ? 8 * c : a0, d1 = is_v ? 8 * c + 4 : a1;
-      if (is_v) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) z[i] = x[i];
-      } else {
-        rope_up4<F16>(y0, z);
-        rope_up4<F16>(y1, z + 4);
-      }
-      float s[Q4<D>::kGroups], m[Q4<D>::kGroups];
-#pragma unroll
-      for (int g = 0; g < Q4<D>::kGroups; ++g) {
-        float lo = INFINITY, hi = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if ((d0 >> 6) == g) q4_range(z[i], lo, hi);
-          if ((d1 >> 6) == g) q4_range(z[4 + i], lo, hi);
-        }
-#pragma unroll
-        for (int t = 1; t < kLanes; t <<= 1) {
-          lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, t));
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, t));
-        }
-        q4_params<F16>(lo, hi, s[g], m[g]);
-      }
-      if (have && slot && !is_q) {
-        uint8_t* tile = static_cast<uint8_t*>(p.cache) + q4_tile<D>(blk, h, Hkv, p.block_size, off);
-        const int j = off % kQ4TileTokens;
-        const int g0 = Q4<D>::kGroups == 1 ? 0 : d0 >> 6, g1 = Q4<D>::kGroups == 1 ? 0 : d1 >> 6;
-        const float s0 = g0 == 0 ? s[0] : s[Q4<D>::kGroups - 1], m0 = g0 == 0 ? m[0] : m[Q4<D>::kGroups - 1];
-        const float s1 = g1 == 0 ? s[0] : s[Q4<D>::kGroups - 1], m1 = g1 == 0 ? m[0] : m[Q4<D>::kGroups - 1];
-        if (is_v) {
-          q4_store_v<D, F16>(tile, j, c, z, s0, m0);
-        } else {
-          q4_store_k4<D>(tile, j, d0, z, s0, m0);
-          q4_store_k4<D>(tile, j, d1, z + 4, s1, m1);
-        }
-        if (c < Q4<D>::kGroups) {
-          const float sp = c == 0 ? s[0] : s[Q4<D>::kGroups - 1], mp = c == 0 ? m[0] : m[Q4<D>::kGroups - 1];
-          q4_store_params<D, F16>(tile, j, is_v ? 1 : 0, c, sp, mp);
-        }
-      }
-    }
   }
 }
 
