@@ -932,23 +932,33 @@ int64_t q4_runs(int64_t tokens) { return (tokens + kQ4TileTokens - 1) / kQ4TileT
 
 template <int D, bool F16, bool TAB32>
 int launch_norm_rope(NormRopeParams p, int64_t tokens, int kind, cudaStream_t st) {
-  constexpr int per_round = kRopeThreads / (D / 8);
+  constexpr int per_round = 32 / (D / 8), warps = kRopeThreads / 32;
   const int rows = p.num_heads + (kind == HCP_ROPE_CACHE_Q4 ? 0 : p.num_kv_heads);
   const int rounds = (rows + per_round - 1) / per_round;
-  // few tokens: one round a block, so the whole token is in flight at once
-  p.spread = tokens * rounds <= 8 * 148 ? rounds : 1;
+  // a warp a token where that fills the card twice over, else its rounds on several
+  const int64_t want = (2 * 148 * kRopeBlocks * warps + tokens - 1) / tokens;
+  p.rounds = static_cast<int>((rounds + std::min<int64_t>(want, rounds) - 1) / std::min<int64_t>(want, rounds));
+  p.parts = (rounds + p.rounds - 1) / p.rounds;
   p.num_tokens = tokens;
-  int64_t grid = tokens * p.spread;
+  int64_t grid = (tokens * p.parts + warps - 1) / warps;
   const int64_t kv_blocks = kind == HCP_ROPE_CACHE_Q4 ? q4_runs(tokens) * p.num_kv_heads : 0;
   grid += kv_blocks;
   if (grid > INT32_MAX) return HCP_ERR_UNSUPPORTED;
   p.kv_blocks = static_cast<unsigned>(kv_blocks);
   const unsigned blocks = static_cast<unsigned>(grid);
-  switch (kind) {
-    case HCP_ROPE_CACHE_SAME: norm_rope_kernel<D, F16, TAB32, kRopeCacheSame><<<blocks, kRopeThreads, 0, st>>>(p); break;
-    case HCP_ROPE_CACHE_Q4: norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4><<<blocks, kRopeThreads, 0, st>>>(p); break;
-    default: norm_rope_kernel<D, F16, TAB32, kRopeCacheNone><<<blocks, kRopeThreads, 0, st>>>(p); break;
-  }
+  auto launch = [&](auto none, auto same, auto q4) {
+    switch (kind) {
+      case HCP_ROPE_CACHE_SAME: same<<<blocks, kRopeThreads, 0, st>>>(p); break;
+      case HCP_ROPE_CACHE_Q4: q4<<<blocks, kRopeThreads, 0, st>>>(p); break;
+      default: none<<<blocks, kRopeThreads, 0, st>>>(p); break;
+    }
+  };
+  if (p.interleaved)
+    launch(norm_rope_kernel<D, F16, TAB32, kRopeCacheNone, true>, norm_rope_kernel<D, F16, TAB32, kRopeCacheSame, true>,
+           norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, true>);
+  else
+    launch(norm_rope_kernel<D, F16, TAB32, kRopeCacheNone, false>, norm_rope_kernel<D, F16, TAB32, kRopeCacheSame, false>,
+           norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, false>);
   return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }
 

@@ -10,9 +10,9 @@
 //
 // Bound by HBM: 2 bytes read and 2 written per element.  D/8 lanes own a row and
 // each lane holds both members of its pairs (4 dims and their 4 partners), so the
-// rotation needs no exchange.  A block works on one token: its lanes load the
-// token's cos / sin once and go over the token's heads, two rows' loads in flight.
-// With few tokens the heads are spread over blocks instead, one round each.  With the
+// rotation needs no exchange.  A warp takes one token: its lanes take the token's
+// cos / sin and the weights into one map and go over the token's heads, three rounds of
+// loads in flight.  With few tokens a token's rounds are spread over warps.  With the
 // 4-bit cache further blocks of the same launch take k and v, 16 tokens of one head
 // each, so that whole tiles of the cache are built in shared memory (q4_cache.cuh).
 #pragma once
@@ -25,6 +25,7 @@
 namespace hcp {
 
 constexpr int kRopeThreads = 128;
+constexpr int kRopeBlocks = 8;   // of an SM
 
 enum : int { kRopeCacheNone = 0, kRopeCacheSame = 1, kRopeCacheQ4 = 2 };
 
@@ -52,20 +53,22 @@ struct NormRopeParams {
   int block_size;
   int bs_shift;
   long long num_tokens;
-  int spread;                  // blocks of a token
+  int parts;                   // warps of a token
+  int rounds;                  // of a warp
   unsigned kv_blocks;          // blocks that take k and v, with the 4-bit cache
 };
 
 template <bool F16>
 __device__ __forceinline__ void rope_up4(const uint2& v, float* x) {
-  x[0] = q4_up<F16>(v.x & 0xffffu);
-  x[1] = q4_up<F16>(v.x >> 16);
-  x[2] = q4_up<F16>(v.y & 0xffffu);
-  x[3] = q4_up<F16>(v.y >> 16);
+  const float2 a = q4_up2<F16>(v.x), b = q4_up2<F16>(v.y);
+  x[0] = a.x;
+  x[1] = a.y;
+  x[2] = b.x;
+  x[3] = b.y;
 }
 template <bool F16>
 __device__ __forceinline__ uint2 rope_down4(const float* x) {
-  return make_uint2(q4_down<F16>(x[0]) | (q4_down<F16>(x[1]) << 16), q4_down<F16>(x[2]) | (q4_down<F16>(x[3]) << 16));
+  return make_uint2(q4_down2<F16>(x[0], x[1]), q4_down2<F16>(x[2], x[3]));
 }
 
 // This lane's dims of a row: a0 .. a0+3 and a1 .. a1+3, partners where it turns them.
@@ -73,16 +76,25 @@ struct RopeLane {
   int a0, a1;
   bool turns;
 };
+template <bool INTER>
 __device__ __forceinline__ RopeLane rope_lane(const NormRopeParams& p, int c) {
   RopeLane r;
   const int pairs = p.rotary / 8;  // lanes that rotate
   r.turns = c < pairs;
-  r.a0 = !r.turns ? p.rotary + 8 * (c - pairs) : p.interleaved ? 8 * c : 4 * c;
-  r.a1 = r.turns && !p.interleaved ? p.rotary / 2 + 4 * c : r.a0 + 4;
+  r.a0 = !r.turns ? p.rotary + 8 * (c - pairs) : INTER ? 8 * c : 4 * c;
+  r.a1 = r.turns && !INTER ? p.rotary / 2 + 4 * c : r.a0 + 4;
   return r;
 }
+// Cosines and sines of the lane's pairs at a position; 1 and 0 where it turns none.
 template <bool F16, bool TAB32>
-__device__ __forceinline__ void rope_angles(const NormRopeParams& p, long long pos, int c, float* cs, float* sn) {
+__device__ __forceinline__ void rope_angles(const NormRopeParams& p, const RopeLane& r, long long pos, int c, float* cs,
+                                            float* sn) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    cs[i] = 1.f;
+    sn[i] = 0.f;
+  }
+  if (!r.turns || pos < 0 || pos >= p.table_rows) return;
   const long long at = pos * p.table_stride + 4 * c;
   if constexpr (TAB32) {
     const float4 a = *reinterpret_cast<const float4*>(static_cast<const float*>(p.table) + at);
@@ -94,53 +106,59 @@ __device__ __forceinline__ void rope_angles(const NormRopeParams& p, long long p
     rope_up4<F16>(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.table) + at + p.rotary / 2), sn);
   }
 }
+// A row's map, weights and rotation in one: with u, v the members of a pair,
+//   u' = inv (u k0 - v k1), v' = inv (v k2 + u k3),  k0 = w_u cos, k1 = w_v sin, k2 = w_v cos, k3 = w_u sin,
+// inv the row's 1 / rms.  One map serves all rows of a token that share the weights.
+struct RopeMap {
+  float k0[4], k1[4], k2[4], k3[4];
+};
+template <bool F16, bool INTER>
+__device__ __forceinline__ void rope_map(RopeMap& f, const RopeLane& r, const uint16_t* w, const float* cs, const float* sn) {
+  float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
+  if (w != nullptr) {
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a0), g);
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a1), g + 4);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float gu = INTER ? g[2 * i] : g[i], gv = INTER ? g[2 * i + 1] : g[4 + i];
+    f.k0[i] = gu * cs[i];
+    f.k1[i] = gv * sn[i];
+    f.k2[i] = gv * cs[i];
+    f.k3[i] = gu * sn[i];
+  }
+}
 // Norm and rotation of one row; every lane of the warp takes part.
-template <int D, bool F16>
-__device__ __forceinline__ void rope_row(const NormRopeParams& p, const RopeLane& r, const uint16_t* w, bool known,
-                                         const float* cs, const float* sn, const uint2 (&in)[2], uint2 (&out)[2]) {
-  float x[8];
+template <int D, bool F16, bool INTER>
+__device__ __forceinline__ void rope_row(const RopeLane& r, const RopeMap& f, bool norm, float eps, const uint2 (&in)[2],
+                                         uint2 (&out)[2]) {
+  float x[8], y[8];
   rope_up4<F16>(in[0], x);
   rope_up4<F16>(in[1], x + 4);
   float sq = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sq += x[i] * x[i];
+  for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
 #pragma unroll
   for (int s = 1; s < D / 8; s <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, s);
-  if (w != nullptr) {
-    const float inv = rsqrtf(sq * (1.f / D) + p.eps);
-    float g[8];
-    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a0), g);
-    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a1), g + 4);
+  const float inv = norm ? rsqrtf(fmaf(sq, 1.f / D, eps)) : 1.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-  }
-  float y[8];
-  if (!r.turns) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
-  } else if (p.interleaved) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[2 * i] = x[2 * i] * cs[i] - x[2 * i + 1] * sn[i];
-      y[2 * i + 1] = x[2 * i + 1] * cs[i] + x[2 * i] * sn[i];
+  for (int i = 0; i < 4; ++i) {
+    const int a = INTER ? 2 * i : i, b = INTER ? 2 * i + 1 : i + 4;
+    y[a] = x[a] * f.k0[i];
+    y[b] = x[b] * f.k2[i];
+    if (r.turns) {  // (the other dims meet no sine: an infinity would not stay in its place)
+      y[a] = fmaf(-x[b], f.k1[i], y[a]);
+      y[b] = fmaf(x[a], f.k3[i], y[b]);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      y[i] = x[i] * cs[i] - x[i + 4] * sn[i];
-      y[i + 4] = x[i + 4] * cs[i] + x[i] * sn[i];
-    }
-  }
-  if (!known) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __int_as_float(0x7fffffff);
+    y[a] *= inv;
+    y[b] *= inv;
   }
   out[0] = rope_down4<F16>(y);
   out[1] = rope_down4<F16>(y + 4);
 }
 
 // k and v of 16 tokens of one head: k normed, rotated and written to k_out, both into the cache.
-template <int D, bool F16, bool TAB32>
+template <int D, bool F16, bool TAB32, bool INTER>
 __device__ __forceinline__ void rope_kv_block(const NormRopeParams& p, int unit, Q4Stage<D>& st) {
   using L = Q4<D>;
   constexpr int kRows = kRopeThreads / L::kLanes;
@@ -161,24 +179,26 @@ __device__ __forceinline__ void rope_kv_block(const NormRopeParams& p, int unit,
     q4_place<D>(st, u, slot, h);
   }
   const int c = threadIdx.x % L::kLanes;
-  const RopeLane ln = rope_lane(p, c);
+  const RopeLane ln = rope_lane<INTER>(p, c);
 #pragma unroll 2
   for (int row = threadIdx.x / L::kLanes; row < kQ4TileTokens; row += kRows) {
     const long long tok = t0 + row;
     const bool here = tok >= 0 && tok < p.num_tokens;
     const long long pos = here ? p.positions[tok] : -1;
-    const bool known = pos < p.table_rows;
     uint2 in[2] = {make_uint2(0u, 0u), make_uint2(0u, 0u)}, out[2];
     uint4 vraw = make_uint4(0u, 0u, 0u, 0u);
-    float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
     if (here) {
       const uint16_t* k = p.k + tok * p.k_stride + static_cast<long long>(h) * D;
       in[0] = *reinterpret_cast<const uint2*>(k + ln.a0);
       in[1] = *reinterpret_cast<const uint2*>(k + ln.a1);
       vraw = reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + static_cast<long long>(h) * D)[c];
     }
-    if (ln.turns && known && pos >= 0) rope_angles<F16, TAB32>(p, pos, c, cs, sn);
-    rope_row<D, F16>(p, ln, p.k_weight, known, cs, sn, in, out);
+    float cs[4], sn[4];
+    rope_angles<F16, TAB32>(p, ln, pos, c, cs, sn);
+    if (pos >= p.table_rows) in[0] = in[1] = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN
+    RopeMap f;
+    rope_map<F16, INTER>(f, ln, p.k_weight, cs, sn);
+    rope_row<D, F16, INTER>(ln, f, p.k_weight != nullptr, p.eps, in, out);
     if (pos >= 0) {
       uint16_t* k = p.k_out + tok * p.k_out_stride + static_cast<long long>(h) * D;
       *reinterpret_cast<uint2*>(k + ln.a0) = out[0];
@@ -217,9 +237,9 @@ __device__ __forceinline__ void rope_kv_block(const NormRopeParams& p, int unit,
     q4_params<F16>(vlo, vhi, vs, vm);
     constexpr int kLast = L::kGroups - 1;
     const bool u0 = ln.a0 < 64, u1 = ln.a1 < 64;
-    q4_stage_k4<D>(st, row, ln.a0, q4_codes<4>(z, u0 ? s[0] : s[kLast], u0 ? m[0] : m[kLast]));
-    q4_stage_k4<D>(st, row, ln.a1, q4_codes<4>(z + 4, u1 ? s[0] : s[kLast], u1 ? m[0] : m[kLast]));
-    q4_stage_v8<D>(st, row, c, q4_codes<8>(x, vs, vm));
+    q4_stage_k4<D>(st, row, ln.a0, q4_codes<4, F16>(z, u0 ? s[0] : s[kLast], u0 ? m[0] : m[kLast]));
+    q4_stage_k4<D>(st, row, ln.a1, q4_codes<4, F16>(z + 4, u1 ? s[0] : s[kLast], u1 ? m[0] : m[kLast]));
+    q4_stage_v8<D>(st, row, c, q4_codes<8, F16>(x, vs, vm));
     if (c < L::kGroups) q4_stage_params<D, F16>(st, row, 0, c, c == 0 ? s[0] : s[kLast], c == 0 ? m[0] : m[kLast]);
     if ((c & 7) == 0) q4_stage_params<D, F16>(st, row, 1, c >> 3, vs, vm);
   }
@@ -228,47 +248,46 @@ __device__ __forceinline__ void rope_kv_block(const NormRopeParams& p, int unit,
 }
 
 // Blocks 0 .. kv_blocks - 1 (with the 4-bit cache; the longer ones come first): k and v, 16
-// tokens of one head each.  The blocks after them: rows of one token each.
-template <int D, bool F16, bool TAB32, int CACHE>
-__global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeParams p) {
+// tokens of one head each.  The warps of the blocks after them: `rounds` rounds of one token's
+// rows each, 32 / (D/8) rows a round, queries before keys.
+template <int D, bool F16, bool TAB32, int CACHE, bool INTER>
+__global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) norm_rope_kernel(const __grid_constant__ NormRopeParams p) {
   constexpr int kLanes = D / 8;
-  constexpr int kRows = kRopeThreads / kLanes;   // rows of a round
-  const int H = p.num_heads, Hkv = p.num_kv_heads;
+  constexpr int kWarpRows = 32 / kLanes;         // rows of a round
+  constexpr int kAhead = 3;                      // rounds in flight
   if constexpr (CACHE == kRopeCacheQ4) {
     __shared__ Q4Stage<D> st;
     if (blockIdx.x < p.kv_blocks) {
-      rope_kv_block<D, F16, TAB32>(p, static_cast<int>(blockIdx.x), st);
+      rope_kv_block<D, F16, TAB32, INTER>(p, static_cast<int>(blockIdx.x), st);
       return;
     }
   }
-  const unsigned bid = blockIdx.x - p.kv_blocks;
-  const unsigned tok32 = p.spread == 1 ? bid : bid / p.spread;
-  const int part = p.spread == 1 ? 0 : bid - tok32 * p.spread;
-  const long long tok = tok32;
-  const int c = threadIdx.x % kLanes;
-  const RopeLane ln = rope_lane(p, c);
+  const int H = p.num_heads, Hkv = p.num_kv_heads;
   const int rows = CACHE == kRopeCacheQ4 ? H : H + Hkv;
-  constexpr int U = 2;
-  uint2 in[U][2], out[2];
-  auto load = [&](int r0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * p.spread * kRows + threadIdx.x / kLanes;
-      in[u][0] = in[u][1] = make_uint2(0u, 0u);
-      if (r < rows) {
-        const uint16_t* row = r < H ? p.q + tok * p.q_stride + static_cast<long long>(r) * D
-                                    : p.k + tok * p.k_stride + static_cast<long long>(r - H) * D;
-        in[u][0] = *reinterpret_cast<const uint2*>(row + ln.a0);
-        in[u][1] = *reinterpret_cast<const uint2*>(row + ln.a1);
-      }
+  const long long unit = static_cast<long long>(blockIdx.x - p.kv_blocks) * (kRopeThreads / 32) + threadIdx.x / 32;
+  const long long tok = p.parts == 1 ? unit : unit / p.parts;
+  if (tok >= p.num_tokens) return;
+  const int part = p.parts == 1 ? 0 : static_cast<int>(unit - tok * p.parts);
+  const int c = threadIdx.x % kLanes, sub = threadIdx.x % 32 / kLanes;
+  const RopeLane ln = rope_lane<INTER>(p, c);
+  // row r stands at base + r * D, for keys too
+  const uint16_t* const qs = p.q + tok * p.q_stride;
+  const uint16_t* const ks = p.k + tok * p.k_stride - static_cast<long long>(H) * D;
+  const int begin = part * p.rounds * kWarpRows, end = min(rows, begin + p.rounds * kWarpRows);
+  uint2 in[kAhead][2], out[2];
+  auto load = [&](uint2 (&to)[2], int r) {
+    to[0] = to[1] = make_uint2(0u, 0u);
+    if (r < end) {
+      const uint16_t* src = (r < H ? qs : ks) + r * D;
+      to[0] = *reinterpret_cast<const uint2*>(src + ln.a0);
+      to[1] = *reinterpret_cast<const uint2*>(src + ln.a1);
     }
   };
-  load(part * kRows);                            // beside the position
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) load(in[i], begin + i * kWarpRows + sub);  // beside the position
   const long long pos = p.positions[tok];
   if (pos < 0) return;                           // padding row: everything stays
   const bool known = pos < p.table_rows;
-  float cs[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
-  if (ln.turns && known) rope_angles<F16, TAB32>(p, pos, c, cs, sn);
   long long dst = -1;                            // cache offset of the token's row of head 0
   if constexpr (CACHE == kRopeCacheSame) {
     long long blk;
@@ -276,33 +295,43 @@ __global__ void __launch_bounds__(kRopeThreads) norm_rope_kernel(const NormRopeP
     if (known && slot_block(p.slot_mapping[tok], p.num_blocks, p.block_size, p.bs_shift, blk, off))
       dst = (blk * Hkv * p.block_size + off) * 2LL * D;
   }
-  for (int r0 = part * kRows; r0 < rows; r0 += p.spread * kRows * U) {
-    if (r0 != part * kRows) load(r0);
+  uint16_t* const qo = p.q_out + tok * p.q_out_stride;
+  uint16_t* const ko = p.k_out + tok * p.k_out_stride - static_cast<long long>(H) * D;
+  bool keys = begin + sub >= H;                  // rows rise: queries' map, then keys'
+  bool norm = (keys ? p.k_weight : p.q_weight) != nullptr;
+  RopeMap f;
+  auto map = [&](const uint16_t* w) {  // (the angles again for the keys: kept, they would cost 8 registers)
+    float cs[4], sn[4];
+    rope_angles<F16, TAB32>(p, ln, pos, c, cs, sn);
+    rope_map<F16, INTER>(f, ln, w, cs, sn);
+  };
+  map(keys ? p.k_weight : p.q_weight);
+  for (int r0 = begin; r0 < end; r0 += kAhead * kWarpRows) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = r0 + u * p.spread * kRows + threadIdx.x / kLanes;
-      if (r0 + u * p.spread * kRows >= rows) break;  // the same for all
-      rope_row<D, F16>(p, ln, r < H ? p.q_weight : p.k_weight, known, cs, sn, in[u], out);
-      if (r >= rows) continue;
-      uint16_t* row = r < H ? p.q_out + tok * p.q_out_stride + static_cast<long long>(r) * D
-                            : p.k_out + tok * p.k_out_stride + static_cast<long long>(r - H) * D;
-      *reinterpret_cast<uint2*>(row + ln.a0) = out[0];
-      *reinterpret_cast<uint2*>(row + ln.a1) = out[1];
+    for (int i = 0; i < kAhead; ++i) {
+      const int r = r0 + i * kWarpRows + sub;
+      if (r0 + i * kWarpRows >= end) break;      // the same for all lanes
+      if (CACHE != kRopeCacheQ4 && !keys && r >= H) {
+        keys = true;
+        norm = p.k_weight != nullptr;
+        map(p.k_weight);
+      }
+      if (!known) in[i][0] = in[i][1] = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN
+      rope_row<D, F16, INTER>(ln, f, norm, p.eps, in[i], out);
+      load(in[i], r + kAhead * kWarpRows);
+      if (r >= end) continue;
+      uint16_t* to = (r < H ? qo : ko) + r * D;
+      *reinterpret_cast<uint2*>(to + ln.a0) = out[0];
+      *reinterpret_cast<uint2*>(to + ln.a1) = out[1];
       if constexpr (CACHE == kRopeCacheSame) {
         if (r >= H && dst >= 0) {
-          uint16_t* to = static_cast<uint16_t*>(p.cache) + dst + static_cast<long long>(r - H) * p.block_size * 2 * D;
-          *reinterpret_cast<uint2*>(to + ln.a0) = out[0];
-          *reinterpret_cast<uint2*>(to + ln.a1) = out[1];
+          uint16_t* at = static_cast<uint16_t*>(p.cache) + dst + static_cast<long long>(r - H) * p.block_size * 2 * D;
+          *reinterpret_cast<uint2*>(at + ln.a0) = out[0];
+          *reinterpret_cast<uint2*>(at + ln.a1) = out[1];
+          reinterpret_cast<uint4*>(at + D)[c] = reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + (r - H) * D)[c];
         }
       }
     }
-  }
-  if constexpr (CACHE == kRopeCacheSame) {
-    if (dst >= 0)
-      for (int h = part * kRows + threadIdx.x / kLanes; h < Hkv; h += p.spread * kRows) {
-        const uint4 v = reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + static_cast<long long>(h) * D)[c];
-        reinterpret_cast<uint4*>(static_cast<uint16_t*>(p.cache) + dst + static_cast<long long>(h) * p.block_size * 2 * D + D)[c] = v;
-      }
   }
 }
 

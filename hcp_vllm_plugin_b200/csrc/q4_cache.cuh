@@ -7,10 +7,9 @@
 //   x'_d = lo + s n_d
 // where round16 rounds to the rows' 16-bit type and round takes ties to even.
 // lo is an element of the group, so it is exact.  s = 0 (a constant group, or a
-// range that underflows) gives n = 0.  A group with an infinity or NaN, or
-// whose range overflows 32 bits, gets s = lo = NaN and reads back as NaN.  All
-// of this is done in 32 bits with IEEE division; n and s are the only rounded
-// values.  4 bits + (16 + 16) / 64 = 4.5 bits an element against 16.
+// range that underflows; s below 2^-126 counts as 0) gives n = 0.  A group with an
+// infinity or NaN, or whose range overflows 32 bits, gets s = lo = NaN and reads back
+// as NaN.  All of this is done in 32 bits; n and s are the only rounded values.  4 bits + (16 + 16) / 64 = 4.5 bits an element against 16.
 //
 // Layout: uint8 [num_blocks, Hkv, block_size, 9 D / 8]; one (block, head) is
 // block_size / 16 tiles of 16 tokens, 18 D bytes each, so a tile is one
@@ -62,20 +61,34 @@ __device__ __forceinline__ uint32_t q4_down(float v) {
   else return __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
 template <bool F16>
+__device__ __forceinline__ float2 q4_up2(uint32_t w) {
+  if constexpr (F16) return __half22float2(*reinterpret_cast<const __half2*>(&w));
+  else return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t q4_down2(float lo, float hi) {
+  if constexpr (F16) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+template <bool F16>
 __device__ __forceinline__ void q4_unpack8(const uint4& v, float (&x)[8]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[2 * i] = q4_up<F16>(w[i] & 0xffffu);
-    x[2 * i + 1] = q4_up<F16>(w[i] >> 16);
+    const float2 f = q4_up2<F16>(w[i]);
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
   }
 }
 template <bool F16>
 __device__ __forceinline__ uint4 q4_pack8(const float (&x)[8]) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = q4_down<F16>(x[2 * i]) | (q4_down<F16>(x[2 * i + 1]) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  return make_uint4(q4_down2<F16>(x[0], x[1]), q4_down2<F16>(x[2], x[3]), q4_down2<F16>(x[4], x[5]),
+                    q4_down2<F16>(x[6], x[7]));
 }
 
 // Packed pairs of the 16-bit type: smallest and largest, NaN wherever one is NaN.
@@ -97,46 +110,56 @@ template <bool F16>
 constexpr uint32_t q4_inf2() { return F16 ? 0x7c007c00u : 0x7f807f80u; }
 
 // Scale and lowest value of a group from the packed ranges of its elements at even
-// and odd places.  The quotient by 15 is the correctly rounded one (reciprocal and
-// one residual, as in q4_codes).  An infinity or NaN in the group, or a range past
-// 32 bits, leaves the residual NaN or the scale infinite.
+// and odd places.  The quotient by 15 is a product corrected by one residual
+// (Markstein), which rounds correctly.  An infinity or NaN in the group, or a range
+// past 32 bits, leaves the residual NaN or the scale infinite.
 template <bool F16>
 __device__ __forceinline__ void q4_params(uint32_t lo2, uint32_t hi2, float& s, float& m) {
-  lo2 = q4_min2<F16>(lo2, lo2 >> 16 | lo2 << 16);
-  hi2 = q4_max2<F16>(hi2, hi2 >> 16 | hi2 << 16);
+  lo2 = q4_min2<F16>(lo2, __byte_perm(lo2, lo2, 0x1032));
+  hi2 = q4_max2<F16>(hi2, __byte_perm(hi2, hi2, 0x1032));
   m = q4_up<F16>(lo2 & 0xffffu);
   const float d = q4_up<F16>(hi2 & 0xffffu) - m;
   constexpr float r = 1.f / 15.f;
   const float q = d * r;
-  s = d < 0x1p-90f ? __fdiv_rn(d, 15.f) : fmaf(fmaf(-q, 15.f, d), r, q);
-  s = q4_up<F16>(q4_down<F16>(s));
+  s = q4_up<F16>(q4_down<F16>(fmaf(fmaf(-q, 15.f, d), r, q)));
+  if (s < 0x1p-126f) s = 0.f;
   if (!(s < INFINITY)) s = m = __int_as_float(0x7fffffff);
 }
+__device__ __forceinline__ float q4_reciprocal(float s) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
+  return r;
+}
 // Whole numbers of N elements of one group, element i in bits 4i..4i+3:
-// round((x - m) / s) as IEEE division and ties to even give it, 0 where s is 0 or NaN.
-// The quotient comes from the correctly rounded reciprocal and one residual
-// (Markstein's theorem: the result is the correctly rounded quotient where nothing
-// under- or overflows); groups near the ends of the exponent range divide.  Adding
-// 2^23 rounds to a whole number, whose bits are the sum's lowest.
-template <int N>
+// round((x - m) / s), ties to even, 0 where s is 0 or NaN.  The quotient is a product
+// with the reciprocal, corrected by one residual (Markstein's step): a quotient that
+// is a tie comes out exact whatever the reciprocal's last bits, and one that is not
+// keeps its side.  Adding 2^23 rounds to a whole number, whose bits are the sum's
+// lowest.  (s is at most 2^128 / 15 and at least 2^-126: its reciprocal is a normal number.)
+template <int N, bool F16>
 __device__ __forceinline__ uint32_t q4_codes(const float* x, float s, float m) {
+  if (!(s > 0.f)) return 0;
+  const float r = q4_reciprocal(s);
+  const float2 r2 = make_float2(r, r), s2 = make_float2(-s, -s), m2 = make_float2(-m, -m), one = make_float2(8388608.f, 8388608.f);
   uint32_t w = 0;
-  if (!(s > 0.f)) return w;
-  if (s > 0x1p-90f && s < 0x1p90f) {
-    const float r = __frcp_rn(s);
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = x[i] - m;
-      const float q = d * r;
-      const float t = fmaf(fmaf(-q, s, d), r, q);
-      w += (__float_as_uint(fminf(t, 15.f) + 8388608.f) - 0x4b000000u) << (4 * i);
+  for (int i = 0; i < N; i += 2) {
+    const float2 d = __fadd2_rn(make_float2(x[i], x[i + 1]), m2);
+    const float2 q = __fmul2_rn(d, r2);
+    float2 t = __ffma2_rn(__ffma2_rn(q, s2, d), r2, q);
+    if (F16) {  // a scale among fp16's smallest numbers may be rounded far down; else t is below 15.5
+      t.x = fminf(t.x, 15.f);
+      t.y = fminf(t.y, 15.f);
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      w += (__float_as_uint(fminf(__fdiv_rn(x[i] - m, s), 15.f) + 8388608.f) - 0x4b000000u) << (4 * i);
+    t = __fadd2_rn(t, one);
+    w += __float_as_uint(t.x) << (4 * i);
+    w += __float_as_uint(t.y) << (4 * i + 4);
   }
-  return w;
+  constexpr uint32_t k2p23 = 0x4b000000u;  // the bits of 2^23, once per element
+  uint32_t all = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) all += k2p23 << (4 * i);
+  return w - all;
 }
 
 // Address of the tile that holds `off` of (block, head).
@@ -299,7 +322,7 @@ __global__ void __launch_bounds__(kQ4Threads) q4_update_kernel(const Q4UpdatePar
       hi = q4_max2<F16>(hi, __shfl_xor_sync(0xffffffffu, hi, k));
     }
     q4_params<F16>(lo, hi, s, m);
-    const uint32_t codes = q4_codes<8>(x, s, m);
+    const uint32_t codes = q4_codes<8, F16>(x, s, m);
     if (is_v) q4_stage_v8<D>(st, j, b, codes);
     else q4_stage_k8<D>(st, j, b, codes);
     if ((b & 7) == 0) q4_stage_params<D, F16>(st, j, is_v ? 1 : 0, b >> 3, s, m);
