@@ -249,6 +249,26 @@ def load(path: str | None = None) -> ctypes.CDLL:
     return lib
 
 
+_front = None
+
+
+def front():
+    """The torch front end of the serving-step entry points, bound to the library."""
+    global _front
+    if _front is None:
+        lib = load()
+        try:
+            from . import _hcp_front as mod
+        except ImportError as e:
+            raise HcpError(f"_hcp_front.so cannot be loaded ({e}): build it for this torch with "
+                           "`python -m hcp_vllm_plugin_b200.build` (there is no fallback)") from e
+        mod.bind(check, *(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "hcp_kv_plan_step", "hcp_qk_norm_rope", "hcp_kv_cache_update_q4", "hcp_kv_cache_gather_q4",
+            "hcp_decode_q4_splitkv", "hcp_decode_q4_workspace_bytes")))
+        _front = mod
+    return _front
+
+
 def check(rc: int, what: str) -> None:
     if rc != HCP_OK:
         raise HcpError(f"{what} failed: {STATUS_NAMES.get(rc, rc)}")

@@ -1,10 +1,12 @@
-"""Build ``libhcp_ring.so`` in-tree with nvcc for sm_100a.
+"""Build ``libhcp_ring.so`` in-tree with nvcc for sm_100a, and ``_hcp_front.so``.
 
     python -m hcp_vllm_plugin_b200.build
 
 The library links the CUDA runtime statically and resolves the driver's
 ``cuTensorMapEncodeTiled`` at run time, so it loads on any box with the
-NVIDIA driver and needs no torch at link time.
+NVIDIA driver and needs no torch at link time.  ``_hcp_front.so`` is the
+torch front end of the serving-step entry points (``csrc/front.cpp``, no
+kernels): an extension module for the installed torch and Python.
 """
 
 from __future__ import annotations
@@ -13,14 +15,17 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhcp_ring.so")
 SOURCES = [os.path.join(CSRC, "hcp_ring.cu")]
-DEPS = SOURCES + [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [
-    os.path.join(ROOT, "include", "hcp_ring.h")]
+HEADER = os.path.join(ROOT, "include", "hcp_ring.h")
+DEPS = SOURCES + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))] + [HEADER]
+FRONT = os.path.join(HERE, "_hcp_front.so")
+FRONT_SOURCE = os.path.join(CSRC, "front.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -41,24 +46,48 @@ def nvcc_path() -> str:
     return found
 
 
-def up_to_date() -> bool:
-    if not os.path.exists(LIB):
+def up_to_date(target: str = LIB, deps=DEPS) -> bool:
+    if not os.path.exists(target):
         return False
-    t = os.path.getmtime(LIB)
-    return all(os.path.getmtime(d) <= t for d in DEPS if os.path.exists(d))
+    t = os.path.getmtime(target)
+    return all(os.path.getmtime(d) <= t for d in deps if os.path.exists(d))
+
+
+def _compile(cmd: list[str], target: str, verbose: bool) -> None:
+    tmp = target + ".tmp"
+    cmd = [tmp if c == target else c for c in cmd]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, target)
+
+
+def build_front(force: bool = False, verbose: bool = False) -> str:
+    """Compile the torch front end with the host compiler."""
+    if not force and up_to_date(FRONT, [FRONT_SOURCE, HEADER]):
+        return FRONT
+    import torch
+
+    home = os.path.dirname(torch.__file__)
+    # of the toolkit the headers alone: no runtime library of it is linked
+    includes = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
+                os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"), sysconfig.get_paths()["include"]]
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+           *(a for p in includes for a in ("-isystem", p)), "-o", FRONT, FRONT_SOURCE,
+           "-L", os.path.join(home, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+           "-ltorch_python"]
+    _compile(cmd, FRONT, verbose)
+    return FRONT
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    tmp = LIB + ".tmp"
-    cmd = [nvcc_path(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC,
-           "-o", tmp, *SOURCES]
-    if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True)
-    os.replace(tmp, LIB)
+    if force or not up_to_date():
+        cmd = [nvcc_path(), *NVCC_FLAGS, "-I", os.path.join(ROOT, "include"), "-I", CSRC, "-o", LIB, *SOURCES]
+        if verbose:
+            cmd.insert(1, "-Xptxas=-v")
+        _compile(cmd, LIB, verbose)
+    build_front(force, verbose)
     return LIB
 
 

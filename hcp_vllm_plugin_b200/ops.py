@@ -437,18 +437,8 @@ def kv_cache_update(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tens
     C.check(rc, "hcp_kv_cache_update")
 
 
-def _vector(t: torch.Tensor, name: str, dtype: torch.dtype, n: int) -> torch.Tensor:
-    """``t`` checked as a contiguous 1-D tensor of ``dtype`` with at least ``n`` entries."""
-    if t.dtype != dtype or t.dim() != 1 or not t.is_contiguous() or t.shape[0] < n:
-        raise ValueError(f"{name} must be a contiguous {dtype} vector of at least {n} entries")
-    return t
-
-
-def _table(t: torch.Tensor, name: str) -> int:
-    """Row stride (elements) of a 2-D table whose rows are contiguous."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
-        raise ValueError(f"{name} must be 2-D with contiguous rows")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+# The serving-step entry points are checked and called in ``csrc/front.cpp``: their
+# kernels take a few microseconds, and these checks in Python as much again.
 
 
 class KvStepPlan(NamedTuple):
@@ -480,39 +470,8 @@ def kv_plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     free_head is not changed: the new head is in the result.  A call repeated on
     the same lengths writes the same entries.
     """
-    _same_device(context_lens, new_lens=new_lens, block_table=block_table, free_blocks=free_blocks,
-                 free_head=free_head, pos_base=pos_base)
-    reqs = context_lens.shape[0]
-    _vector(context_lens, "context_lens", torch.int32, 0)
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < reqs:
-        raise ValueError("block_table must be an int32 [num_reqs, max_blocks] tensor")
-    a = C.HcpStepPlanArgs()
-    a.context_lens, a.new_lens = _ptr(context_lens), _ptr(_vector(new_lens, "new_lens", torch.int32, reqs))
-    if pos_base is not None:
-        a.pos_base = _ptr(_vector(pos_base, "pos_base", torch.int32, reqs))
-    a.block_table, a.block_table_stride = _ptr(block_table), _table(block_table, "block_table")
-    a.block_table_width = block_table.shape[1]
-    a.free_blocks = _ptr(_vector(free_blocks, "free_blocks", torch.int32, 0))
-    a.num_free = free_blocks.shape[0]
-    a.free_head = _ptr(_vector(free_head, "free_head", torch.int32, 1))
-    if num_tokens < 0 or block_size <= 0:
-        raise ValueError("num_tokens must be >= 0 and block_size positive")
-    dev = context_lens.device
-    wide = torch.empty(2 * num_tokens, dtype=torch.int64, device=dev)
-    small = torch.empty(2 * reqs + 2 * num_tokens + 3, dtype=torch.int32, device=dev)
-    at, at64 = _ptr(small), _ptr(wide)
-    a.positions, a.slot_mapping = at64, at64 + 8 * num_tokens
-    a.query_start, a.seq_lens = at, at + 4 * (reqs + 1)
-    a.token_req = at + 4 * (2 * reqs + 1)
-    a.kv_lens = a.token_req + 4 * num_tokens
-    a.free_head_out, a.missing_out = a.kv_lens + 4 * num_tokens, a.kv_lens + 4 * num_tokens + 4
-    a.num_reqs, a.block_size, a.num_tokens = reqs, int(block_size), int(num_tokens)
-    with _dev(context_lens):
-        C.check(C.load().hcp_kv_plan_step(ctypes.byref(a), _stream(context_lens)), "hcp_kv_plan_step")
-    # the views are made while the kernel runs
-    positions, slots = wide.split_with_sizes([num_tokens, num_tokens])
-    start, lens, req, kv, head, missing = small.split_with_sizes([reqs + 1, reqs, num_tokens, num_tokens, 1, 1])
-    return KvStepPlan(start, lens, positions, slots, req, kv, head, missing)
+    return KvStepPlan._make(C.front().plan_step(context_lens, new_lens, block_table, free_blocks, free_head, block_size,
+                                                num_tokens, pos_base))
 
 
 def kv_cache_q4_shape(num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int) -> tuple[int, ...]:
@@ -520,18 +479,6 @@ def kv_cache_q4_shape(num_blocks: int, num_kv_heads: int, block_size: int, head_
     if head_dim not in (64, 128) or block_size not in (16, 32, 64, 128):
         raise ValueError("the 4-bit cache takes head_dim 64 or 128 and block_size 16, 32, 64 or 128")
     return num_blocks, num_kv_heads, block_size, 9 * head_dim // 8
-
-
-def _q4_cache(kv_cache: torch.Tensor, num_kv_heads: int | None, head_dim: int | None) -> int:
-    """Head size of a 4-bit cache, checked against the rows' (where given)."""
-    if kv_cache.dim() != 4 or kv_cache.dtype != torch.uint8 or not kv_cache.is_contiguous():
-        raise ValueError("kv_cache must be a contiguous uint8 [num_blocks, Hkv, block_size, 9*D/8] tensor")
-    d = kv_cache.shape[3] * 8 // 9
-    if 9 * d != kv_cache.shape[3] * 8 or (head_dim is not None and d != head_dim):
-        raise ValueError(f"kv_cache's last dimension {kv_cache.shape[3]} is not 9*D/8 of the rows' head size")
-    if num_kv_heads is not None and kv_cache.shape[1] != num_kv_heads:
-        raise ValueError(f"kv_cache holds {kv_cache.shape[1]} KV heads, the rows {num_kv_heads}")
-    return d
 
 
 def kv_cache_update_q4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.Tensor,
@@ -543,20 +490,7 @@ def kv_cache_update_q4(key: torch.Tensor, value: torch.Tensor, kv_cache: torch.T
     kept as 16 even steps between their smallest and largest element; groups with
     an infinity or NaN read back as NaN.  The slots of a call must be distinct.
     """
-    _same_device(key, value=value, kv_cache=kv_cache, slot_mapping=slot_mapping)
-    if key.dtype not in (torch.bfloat16, torch.float16) or value.dtype != key.dtype or key.shape != value.shape:
-        raise ValueError("key and value must be bf16 or fp16 rows of one shape")
-    if key.dim() != 3:
-        raise ValueError(f"key must be [rows, heads, head_dim], got {tuple(key.shape)}")
-    _q4_cache(kv_cache, key.shape[1], key.shape[2])
-    _vector(slot_mapping, "slot_mapping", torch.int64, 0)
-    n = min(slot_mapping.shape[0], key.shape[0])
-    with _dev(key):
-        rc = C.load().hcp_kv_cache_update_q4(
-            _ptr(key), _ptr(value), n, _rows_heads(key, "key"), _rows_heads(value, "value"), _ptr(slot_mapping),
-            _ptr(kv_cache), kv_cache.shape[0], kv_cache.shape[2], key.shape[1], key.shape[2], _DT[key.dtype],
-            _stream(key))
-    C.check(rc, "hcp_kv_cache_update_q4")
+    C.front().update_q4(key, value, kv_cache, slot_mapping)
 
 
 def kv_cache_gather_q4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, dtype: torch.dtype,
@@ -566,25 +500,7 @@ def kv_cache_gather_q4(kv_cache: torch.Tensor, slot_mapping: torch.Tensor, dtype
     they were written in (``hcp_kv_cache_gather_q4``); rows :func:`ring_attn_fwd`
     takes as contiguous keys.  Otherwise as :func:`kv_cache_gather`.
     """
-    _same_device(kv_cache, slot_mapping=slot_mapping, key=key, value=value)
-    if dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError(f"unsupported dtype {dtype}")
-    d = _q4_cache(kv_cache, None, None)
-    nb, hkv, bs, _ = kv_cache.shape
-    n = _vector(slot_mapping, "slot_mapping", torch.int64, 0).shape[0]
-    if key is None:
-        key = torch.empty(n, hkv, d, dtype=dtype, device=kv_cache.device)
-    if value is None:
-        value = torch.empty(n, hkv, d, dtype=dtype, device=kv_cache.device)
-    for name, t in (("key", key), ("value", value)):
-        if t.dim() != 3 or t.shape[0] < n or tuple(t.shape[1:]) != (hkv, d) or t.dtype != dtype:
-            raise ValueError(f"{name} must hold n rows [Hkv, D] of {dtype}")
-    with _dev(kv_cache):
-        rc = C.load().hcp_kv_cache_gather_q4(
-            _ptr(kv_cache), nb, bs, hkv, d, _ptr(slot_mapping), n, _ptr(key), _ptr(value),
-            _rows_heads(key, "key"), _rows_heads(value, "value"), _DT[dtype], _stream(kv_cache))
-    C.check(rc, "hcp_kv_cache_gather_q4")
-    return key, value
+    return C.front().gather_q4(kv_cache, slot_mapping, dtype, key, value)
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor, *,
@@ -608,55 +524,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     Rows with a negative position are padding and stay as they were; positions
     past the table give NaN rows and write no slot.
     """
-    _same_device(q, k=k, positions=positions, cos_sin=cos_sin, q_weight=q_weight, k_weight=k_weight, q_out=q_out,
-                 k_out=k_out, value=value, kv_cache=kv_cache, slot_mapping=slot_mapping)
-    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype:
-        raise ValueError("q and k must be bf16 or fp16 rows of one dtype")
-    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError("q must be [T, H, D] and k [T, Hkv, D]")
-    tokens, heads, d = q.shape
-    if cos_sin.dtype not in (torch.float32, q.dtype):
-        raise ValueError("cos_sin must be float32 or q's dtype")
-    if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    for name, t, like in (("q_out", q_out, q), ("k_out", k_out, k)):
-        if t.shape != like.shape or t.dtype != q.dtype:
-            raise ValueError(f"{name} must have the shape and dtype of {name[0]}")
-    for name, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if t is not None:
-            _vector(t, name, q.dtype, d)
-    a = C.HcpNormRopeArgs()
-    a.dtype, a.num_heads, a.num_kv_heads, a.head_dim = _DT[q.dtype], heads, k.shape[1], d
-    a.q, a.q_row_stride, a.k, a.k_row_stride = _ptr(q), _rows_heads(q, "q"), _ptr(k), _rows_heads(k, "k")
-    a.q_out, a.q_out_row_stride = _ptr(q_out), _rows_heads(q_out, "q_out")
-    a.k_out, a.k_out_row_stride = _ptr(k_out), _rows_heads(k_out, "k_out")
-    a.positions, a.num_tokens = _ptr(_vector(positions, "positions", torch.int64, tokens)), tokens
-    a.cos_sin, a.table_stride, a.table_rows = _ptr(cos_sin), _table(cos_sin, "cos_sin"), cos_sin.shape[0]
-    a.table_dtype, a.rotary, a.interleaved, a.eps = _DT[cos_sin.dtype], cos_sin.shape[1], bool(interleaved), float(eps)
-    a.q_weight, a.k_weight = _ptr(q_weight), _ptr(k_weight)
-    if kv_cache is not None:
-        if value is None or slot_mapping is None:
-            raise ValueError("kv_cache needs value and slot_mapping")
-        if value.shape != k.shape or value.dtype != k.dtype:
-            raise ValueError("value must have k's shape and dtype")
-        a.v, a.v_row_stride = _ptr(value), _rows_heads(value, "value")
-        if kv_cache.dtype == torch.uint8:
-            _q4_cache(kv_cache, k.shape[1], d)
-            a.cache_kind = C.HCP_ROPE_CACHE_Q4
-        else:
-            if (kv_cache.dim() != 4 or not kv_cache.is_contiguous() or kv_cache.dtype != q.dtype
-                    or kv_cache.shape[1] != k.shape[1] or kv_cache.shape[3] != 2 * d):
-                raise ValueError("kv_cache must be a contiguous [num_blocks, Hkv, block_size, 2*D] tensor")
-            a.cache_kind = C.HCP_ROPE_CACHE_SAME
-        a.kv_cache, a.num_blocks, a.block_size = _ptr(kv_cache), kv_cache.shape[0], kv_cache.shape[2]
-        a.slot_mapping = _ptr(_vector(slot_mapping, "slot_mapping", torch.int64, tokens))
-    elif value is not None or slot_mapping is not None:
-        raise ValueError("value and slot_mapping go with kv_cache")
-    with _dev(q):
-        C.check(C.load().hcp_qk_norm_rope(ctypes.byref(a), _stream(q)), "hcp_qk_norm_rope")
-    return q_out, k_out
+    return C.front().norm_rope(q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out, value,
+                               kv_cache, slot_mapping)
 
 
 def decode_splitkv_q4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor, *,
@@ -673,45 +542,4 @@ def decode_splitkv_q4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torc
     they were.  Peer keys in 16 bits are joined by :func:`decode_splitkv` and
     :func:`merge_attn_states`.
     """
-    if not q.is_cuda or q.dtype not in (torch.bfloat16, torch.float16):
-        raise ValueError("q must be a bf16/fp16 CUDA tensor (no CPU path)")
-    _same_device(q, kv_cache=kv_cache, block_table=block_table, kv_lens=kv_lens, out=out, lse=lse,
-                 token_req=token_req, workspace=workspace)
-    if q.dim() != 3:
-        raise ValueError(f"q must be [rows, heads, head_dim], got {tuple(q.shape)}")
-    rows, heads, d = q.shape
-    _q4_cache(kv_cache, None, d)
-    if block_table.dtype != torch.int32:
-        raise ValueError("block_table must be an int32 [num_reqs, max_blocks] tensor")
-    if out.dim() != 3 or out.shape[0] < rows or out.shape[1:] != q.shape[1:] or out.dtype not in (q.dtype, torch.float32):
-        raise ValueError("out must be [>= q rows, H, D] of q's dtype or float32")
-    a = C.HcpDecodeQ4Args()
-    a.dtype, a.num_heads, a.num_kv_heads, a.head_dim = _DT[q.dtype], heads, kv_cache.shape[1], d
-    a.scale, a.block_size = float(scale), kv_cache.shape[2]
-    a.q, a.q_rows, a.q_row_stride = _ptr(q), rows, _rows_heads(q, "q")
-    a.kv_cache, a.num_blocks = _ptr(kv_cache), kv_cache.shape[0]
-    a.block_table, a.block_table_stride = _ptr(block_table), _table(block_table, "block_table")
-    a.block_table_rows, a.block_table_width = block_table.shape
-    a.kv_lens = _ptr(_vector(kv_lens, "kv_lens", torch.int32, rows))
-    if token_req is not None:
-        a.token_req = _ptr(_vector(token_req, "token_req", torch.int32, rows))
-    elif block_table.shape[0] < rows:
-        raise ValueError("block_table needs a row for every query row (or token_req)")
-    a.out, a.out_dtype, a.out_row_stride = _ptr(out), _DT[out.dtype], _rows_heads(out, "out")
-    if lse is not None:
-        if (lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] != heads or lse.shape[1] < rows
-                or (lse.shape[1] > 1 and lse.stride(1) != 1)):
-            raise ValueError("lse must be a float32 [H, >= q rows] tensor with unit column stride")
-        a.lse, a.lse_stride = _ptr(lse), lse.stride(0) if heads > 1 else lse.shape[1]
-    lib = C.load()
-    need = lib.hcp_decode_q4_workspace_bytes(ctypes.byref(a))
-    if need < 0:
-        raise C.HcpError("hcp_decode_q4_workspace_bytes: invalid arguments")
-    # a buffer of its own per call: torch's allocator orders its reuse on the
-    # stream, and a captured call keeps its own with the graph
-    ws = workspace if workspace is not None else torch.empty(need, dtype=torch.uint8, device=q.device)
-    if not ws.is_contiguous():
-        raise ValueError("workspace must be contiguous")
-    a.workspace, a.workspace_bytes = _ptr(ws), ws.numel() * ws.element_size()
-    with _dev(q):
-        C.check(lib.hcp_decode_q4_splitkv(ctypes.byref(a), _stream(q)), "hcp_decode_q4_splitkv")
+    C.front().decode_q4(q, kv_cache, block_table, kv_lens, scale, out, lse, token_req, workspace)

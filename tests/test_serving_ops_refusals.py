@@ -122,9 +122,9 @@ def test_decode_q4_refusals(lib, over, want):
 
 
 def test_decode_q4_workspace(lib):
-    """The workspace's size depends on the heads alone; one that is missing, short or misaligned is refused."""
+    """The workspace's size depends on rows and heads, on no length; one that is missing, short or misaligned is refused."""
     need = lib.hcp_decode_q4_workspace_bytes(ctypes.byref(_args(C.HcpDecodeQ4Args, DECODE, {})))
-    for over in (dict(q_rows=2), dict(num_blocks=10000), dict(block_table_width=5000, block_table_stride=5000)):
+    for over in (dict(num_blocks=10000), dict(block_table_width=5000, block_table_stride=5000)):
         assert lib.hcp_decode_q4_workspace_bytes(ctypes.byref(_args(C.HcpDecodeQ4Args, DECODE, over))) == need
     for over in (dict(workspace=None), dict(workspace_bytes=need - 1), dict(workspace=_addr(7) + 8)):
         assert lib.hcp_decode_q4_splitkv(ctypes.byref(_args(C.HcpDecodeQ4Args, DECODE, over)), None) == INVALID
