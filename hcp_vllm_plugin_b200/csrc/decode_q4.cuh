@@ -678,37 +678,39 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
   }
 }
 
-// Joins the parts of (row, KV head) blockIdx.x.  Few pairs have many parts each: then a
-// block takes one head (blockIdx.y) and its warps share the parts; else each warp takes heads
-// of its own and all their parts.  Sums run in a fixed order either way.
-template <int D, bool SHARE>
-__global__ void __launch_bounds__(kDq4JoinWarps * 32, 2) decode_q4_join_kernel(const __grid_constant__ DecodeQ4Params p) {
+// Joins the parts of (row, KV head) blockIdx.x; sums run in a fixed order.
+__device__ __forceinline__ bool dq4_parts(const DecodeQ4Params& p, int4& desc) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 desc = p.desc[blockIdx.x];
-  if (desc.z <= 0 || desc.x < 0 || desc.x + desc.z > kDq4MaxPieces || (desc.y & ~1) != 0) return;
+  desc = p.desc[blockIdx.x];
+  return desc.z > 0 && desc.x >= 0 && desc.x + desc.z <= kDq4MaxPieces && (desc.y & ~1) == 0;
+}
+__device__ __forceinline__ long long dq4_part(const int4& desc, int i, int G, int h) {
+  return (static_cast<long long>(desc.x + i) * 2 + (i == 0 ? desc.y : 0)) * G + h;
+}
+__device__ __forceinline__ float dq4_lse(float M, float ls) {
+  return ls == 0.f ? -INFINITY : (M + lg2_approx(ls)) * 0.69314718055994530942f;
+}
+
+// Many pairs, each of few parts: a warp takes a head of the pair and all its parts.
+template <int D>
+__global__ void __launch_bounds__(256) decode_q4_join_kernel(const __grid_constant__ DecodeQ4Params p) {
+  int4 desc;
+  if (!dq4_parts(p, desc)) return;
   constexpr int V = D / 32;  // neighbouring dims of a lane
-  const int G = p.group, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int G = p.group, lane = threadIdx.x & 31;
   const int row = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
-  __shared__ float so[SHARE ? kDq4JoinWarps : 1][D], sl[kDq4JoinWarps], smx[kDq4JoinWarps];
-  for (int h = SHARE ? blockIdx.y : warp; h < G; h += SHARE ? gridDim.y : warps) {
-    auto index = [&](int i) { return (static_cast<long long>(desc.x + i) * 2 + (i == 0 ? desc.y : 0)) * G + h; };
+  for (int h = threadIdx.x >> 5; h < G; h += blockDim.x >> 5) {
     float M = -INFINITY;
-    for (int i = SHARE ? static_cast<int>(threadIdx.x) : lane; i < desc.z; i += SHARE ? static_cast<int>(blockDim.x) : 32)
-      M = fmaxf(M, p.part_ml[index(i)].x);
+    for (int i = lane; i < desc.z; i += 32) M = fmaxf(M, p.part_ml[dq4_part(desc, i, G, h)].x);
 #pragma unroll
     for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-    if constexpr (SHARE) {
-      if (lane == 0) smx[warp] = M;
-      __syncthreads();
-      for (int w = 0; w < warps; ++w) M = fmaxf(M, smx[w]);
-    }
     float acc[V], ls = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) acc[v] = 0.f;
     if (M != -INFINITY) {
 #pragma unroll 8
-      for (int i = SHARE ? warp : 0; i < desc.z; i += SHARE ? warps : 1) {
-        const long long at = index(i);
+      for (int i = 0; i < desc.z; ++i) {
+        const long long at = dq4_part(desc, i, G, h);
         const float2 ml = p.part_ml[at];
         const float x = ex2_approx(ml.x - M);
         ls = fmaf(x, ml.y, ls);
@@ -727,26 +729,88 @@ __global__ void __launch_bounds__(kDq4JoinWarps * 32, 2) decode_q4_join_kernel(c
       }
     }
     const int head = kvh * G + h;
-    if constexpr (SHARE) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) so[warp][V * lane + v] = acc[v];
-      if (lane == 0) sl[warp] = ls;
-      __syncthreads();
-      ls = 0.f;
-      for (int w = 0; w < warps; ++w) ls += sl[w];
-      for (int d = threadIdx.x; d < D; d += blockDim.x) {
-        float v = 0.f;
-        for (int w = 0; w < warps; ++w) v += so[w][d];
-        dq4_store(p, row, head, D, d, ls == 0.f ? 0.f : v / ls);
-      }
-      __syncthreads();
-    } else {
-#pragma unroll
-      for (int v = 0; v < V; ++v) dq4_store(p, row, head, D, V * lane + v, ls == 0.f ? 0.f : acc[v] / ls);
-    }
-    if ((SHARE ? threadIdx.x : lane) == 0 && p.lse != nullptr)
-      p.lse[head * p.lse_stride + row] = ls == 0.f ? -INFINITY : (M + lg2_approx(ls)) * 0.69314718055994530942f;
+    for (int v = 0; v < V; ++v) dq4_store(p, row, head, D, V * lane + v, ls == 0.f ? 0.f : acc[v] / ls);
+    if (lane == 0 && p.lse != nullptr) p.lse[head * p.lse_stride + row] = dq4_lse(M, ls);
   }
+}
+
+// Few pairs, each of many parts: a block takes 32 V dims (blockIdx.z) of one head (blockIdx.y) and
+// its warps share the parts, P each at a time, all loaded before the first weight is known.  The
+// parts were just written by other SMs, so the reads' latency is what this costs.
+template <int D, int V, int P>
+__global__ void __launch_bounds__(kDq4JoinWarps * 32) decode_q4_join_wide_kernel(const __grid_constant__ DecodeQ4Params p) {
+  int4 desc;
+  if (!dq4_parts(p, desc)) return;
+  __shared__ float weight[kDq4MaxPieces], red[kDq4JoinWarps], sum[kDq4JoinWarps], so[kDq4JoinWarps][32 * V];
+  const int G = p.group, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  const float* const part = p.part_o + (blockIdx.z * 32 + lane) * V;
+  float o[P][V];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      const int i = i0 + j * warps;
+#pragma unroll
+      for (int v = 0; v < V; ++v) o[j][v] = 0.f;
+      if (i >= desc.z) continue;
+      const float* at = part + dq4_part(desc, i, G, h) * D;
+      if constexpr (V == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(at);
+        o[j][0] = x.x; o[j][1] = x.y; o[j][2] = x.z; o[j][3] = x.w;
+      } else if constexpr (V == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(at);
+        o[j][0] = x.x; o[j][1] = x.y;
+      } else {
+        o[j][0] = *at;
+      }
+    }
+  };
+  load(warp);
+  float M = -INFINITY;
+  for (int i = tid; i < desc.z; i += blockDim.x) M = fmaxf(M, p.part_ml[dq4_part(desc, i, G, h)].x);
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+  if (lane == 0) red[warp] = M;
+  __syncthreads();
+  M = red[0];
+  for (int w = 1; w < warps; ++w) M = fmaxf(M, red[w]);
+  const float base = M == -INFINITY ? 0.f : M;
+  float ls = 0.f;
+  for (int i = tid; i < desc.z; i += blockDim.x) {
+    const float2 ml = p.part_ml[dq4_part(desc, i, G, h)];
+    const float x = ex2_approx(ml.x - base);
+    weight[i] = x;
+    ls = fmaf(x, ml.y, ls);
+  }
+#pragma unroll
+  for (int s = 16; s > 0; s >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, s);
+  if (lane == 0) sum[warp] = ls;
+  __syncthreads();
+  float acc[V];
+#pragma unroll
+  for (int v = 0; v < V; ++v) acc[v] = 0.f;
+  for (int i0 = warp; i0 < desc.z; i0 += P * warps) {
+    if (i0 != warp) load(i0);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      if (i0 + j * warps >= desc.z) break;
+      const float x = weight[i0 + j * warps];
+#pragma unroll
+      for (int v = 0; v < V; ++v) acc[v] = fmaf(x, o[j][v], acc[v]);
+    }
+  }
+#pragma unroll
+  for (int v = 0; v < V; ++v) so[warp][lane * V + v] = acc[v];
+  __syncthreads();
+  const int row = blockIdx.x / p.num_kv_heads, head = blockIdx.x % p.num_kv_heads * G + h;
+  ls = 0.f;
+  for (int w = 0; w < warps; ++w) ls += sum[w];
+  for (int d = tid; d < 32 * V; d += blockDim.x) {
+    float v = 0.f;
+    for (int w = 0; w < warps; ++w) v += so[w][d];
+    dq4_store(p, row, head, D, blockIdx.z * 32 * V + d, ls == 0.f ? 0.f : v / ls);
+  }
+  if (tid == 0 && blockIdx.z == 0 && p.lse != nullptr) p.lse[head * p.lse_stride + row] = dq4_lse(M, ls);
 }
 
 }  // namespace hcp

@@ -916,6 +916,7 @@ extern "C" int hcp_kv_plan_step(const hcp_step_plan_args* a, void* stream) {
   p.num_reqs = a->num_reqs;
   p.num_tokens = a->num_tokens;
   p.block_size = a->block_size;
+  p.bs_shift = pow2_shift(a->block_size);
   const int64_t blocks = std::max<int64_t>(1, (a->num_tokens + kPlanThreads - 1) / kPlanThreads);
   step_plan_kernel<<<static_cast<int>(std::min<int64_t>(blocks, 2 * 148)), kPlanThreads, 0,
                      static_cast<cudaStream_t>(stream)>>>(p);
@@ -982,21 +983,22 @@ int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
   if (cudaGetLastError() != cudaSuccess) return HCP_ERR_CUDA;
   // the joining kernel may start while the first one ends; it waits for it itself
   const int64_t pairs = static_cast<int64_t>(p.rows) * p.num_kv_heads;
-  const bool share = pairs <= kDq4Sms;  // one pair or a few an SM: their parts are shared between warps
+  const int64_t parts = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps / pairs + 2;  // of a pair, were the rows alike
+  // From about 16 parts on they are shared between warps, 8 each; where the heads alone leave SMs
+  // idle, a head's dims are split over blocks too (parts are many then).
+  const bool wide = parts >= 16, split = pairs * p.group < kDq4Sms;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(pairs), share ? static_cast<unsigned>(p.group) : 1u);
-  // parts of a pair, were the rows alike: 8 a warp, which loads them at once
-  const int64_t parts = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps / pairs + 2;
-  const int warps = share ? static_cast<int>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8)) : std::min(p.group, 8);
-  cfg.blockDim = dim3(32 * warps);
+  cfg.gridDim = dim3(static_cast<unsigned>(pairs), wide ? static_cast<unsigned>(p.group) : 1u, split ? D / 32 : 1);
+  cfg.blockDim = dim3(32 * (wide ? static_cast<int>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8)) : std::min(p.group, 8)));
   cfg.stream = st;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = share ? cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D, true>, p)
-                              : cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D, false>, p);
+  const cudaError_t e = !wide ? cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D>, p)
+                        : split ? cudaLaunchKernelEx(&cfg, decode_q4_join_wide_kernel<D, 1, 32>, p)
+                                : cudaLaunchKernelEx(&cfg, decode_q4_join_wide_kernel<D, D / 32, 8>, p);
   return e == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
 }
 

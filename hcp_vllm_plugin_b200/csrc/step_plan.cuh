@@ -48,10 +48,16 @@ struct StepPlanParams {
   int num_reqs;
   long long num_tokens;
   int block_size;
+  int bs_shift;                // log2(block_size) when it is a power of two, else -1
 };
 
+// n / block_size for n >= 0 (a 64-bit division costs more than the rest of a request)
+__device__ __forceinline__ long long plan_blocks(const StepPlanParams& p, long long n) {
+  return p.bs_shift >= 0 ? n >> p.bs_shift : n / p.block_size;
+}
+
 struct PlanReq {
-  long long ctx, add, have, need;
+  long long ctx, add, have, want, need;
 };
 
 __device__ __forceinline__ int plan_i32(long long v) {
@@ -62,9 +68,9 @@ __device__ __forceinline__ PlanReq plan_req(const StepPlanParams& p, int r) {
   PlanReq q;
   q.ctx = max(0, p.context_lens[r]);
   q.add = max(0, p.new_lens[r]);
-  q.have = (q.ctx + p.block_size - 1) / p.block_size;
-  const long long want = (q.ctx + q.add + p.block_size - 1) / p.block_size;
-  q.need = max(0ll, min(want, p.bt_width) - q.have);
+  q.have = plan_blocks(p, q.ctx + p.block_size - 1);
+  q.want = plan_blocks(p, q.ctx + q.add + p.block_size - 1);
+  q.need = max(0ll, min(q.want, p.bt_width) - q.have);
   return q;
 }
 
@@ -76,11 +82,12 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanP
   const int run = (p.num_reqs + kPlanThreads - 1) / kPlanThreads;
   const int r0 = min(p.num_reqs, tid * run), r1 = min(p.num_reqs, r0 + run);
   long long tok = 0, blk = 0, wanted = 0;
+#pragma unroll 4
   for (int r = r0; r < r1; ++r) {
     const PlanReq q = plan_req(p, r);
     tok += q.add;
     blk += q.need;
-    wanted += max(0ll, (q.ctx + q.add + p.block_size - 1) / p.block_size - q.have);
+    wanted += q.want - q.have;
   }
   long long it = tok, ib = blk;
 #pragma unroll
@@ -176,7 +183,7 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanP
       q = plan_req(p, ++r);
     }
     const long long pos = q.ctx + (t - base);
-    const long long idx = pos / p.block_size;
+    const long long idx = plan_blocks(p, pos);
     int page = -1;
     if (idx < p.bt_width) {
       if (idx < q.have) {
