@@ -678,6 +678,69 @@ def test_two_captured_decodes_do_not_share_partials(ops):
         torch.cuda.synchronize()
 
 
+def test_a_captured_16_bit_decode_keeps_its_partials(ops):
+    """Streams can be captured by every entry point; a captured split-KV decode keeps the buffer of
+    its partials when a later call needs a larger one, and a graph's buffer serves no other call."""
+    gen = torch.Generator().manual_seed(27)
+    h, hkv, d, keys = 28, 4, 128, 6000
+
+    def problem(n):
+        q = _randn(gen, n, h, d).cuda()
+        k, v = _randn(gen, n * keys, hkv, d).cuda(), _randn(gen, n * keys, hkv, d).cuda()
+        return q, k, v, np.array([(i, i * keys, keys, -1, 0, 0) for i in range(n)], np.int32), torch.zeros_like(q)
+
+    run = lambda q, k, v, s, out: ops.decode_splitkv(q, s, scale=0.1, num_kv_heads=hkv, out=out, peer_k=k, peer_v=v)  # noqa: E731
+    small, large = problem(2), problem(40)
+    run(*small)
+    want = small[4].clone()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run(*small)
+        graphs.append(g)
+    run(*large)
+    ref = large[4].clone()
+    junk = [torch.full((1 << 20,), 0xFF, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    for g in graphs:
+        small[4].zero_()
+        g.replay()
+        run(*large)
+        torch.cuda.synchronize()
+        assert torch.equal(small[4], want) and torch.equal(large[4], ref)
+    del junk
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured ones: nothing has to be warmed up."""
+    import subprocess
+    import sys
+    code = """
+import torch
+from hcp_vllm_plugin_b200 import ops
+cache = torch.zeros(ops.kv_cache_q4_shape(4, 2, 16, 128), dtype=torch.uint8, device="cuda")
+i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+table, free, head, ctx, new = i32(*([-1] * 4)).view(2, 2), i32(0, 1, 2, 3), i32(0), i32(0, 0), i32(5, 3)
+q, k, v = (torch.randn(8, n, 128, device="cuda").bfloat16() for n in (4, 2, 2))
+tab = torch.cat([torch.ones(9, 64, device="cuda"), torch.zeros(9, 64, device="cuda")], -1)
+out = torch.zeros_like(q)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    plan = ops.kv_plan_step(ctx, new, table, free, head, block_size=16, num_tokens=8)
+    qr, kr = ops.qk_norm_rope(q, k, plan.positions, tab, value=v, kv_cache=cache, slot_mapping=plan.slot_mapping)
+    ops.decode_splitkv_q4(qr, cache, table, plan.kv_lens, scale=0.1, out=out, token_req=plan.token_req)
+    kc, vc = ops.kv_cache_gather_q4(cache, plan.slot_mapping, torch.bfloat16)
+g.replay()
+torch.cuda.synchronize()
+assert table[:, 0].tolist() == [0, 1] and (vc - v).abs().max() < 0.6
+assert (out[0].view(2, 2, 128) - vc[0][:, None]).abs().max() < 0.05   # the first row sees one key
+print("captured first")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured first" in r.stdout, r.stderr[-2000:]
+
+
 def test_q4_decode_joins_a_peer_partial(ops):
     """Local keys in 4 bits, peer keys in 16: each with its LSE, joined by merge_attn_states."""
     gen = torch.Generator().manual_seed(24)
