@@ -200,6 +200,7 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
   const int g = lane >> 2, t = lane & 3;
   const int G = p.group, Hkv = p.num_kv_heads;
   const Q4Consts consts = q4_consts();
+  ptx::chain_wait();
 
   // ---- the line of tiles: sums of every thread's run of rows
   const int run = (p.rows + kDq4Threads - 1) / kDq4Threads;
@@ -223,7 +224,7 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     before += w < warp ? sm.wsum[w] : 0;
     all += sm.wsum[w];
   }
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  ptx::chain_next();
 
   // ---- the warps' pieces of the line; the thread whose rows hold a piece's first tile says where
   constexpr int kPieces = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps;
@@ -680,7 +681,8 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
 
 // Joins the parts of (row, KV head) blockIdx.x; sums run in a fixed order.
 __device__ __forceinline__ bool dq4_parts(const DecodeQ4Params& p, int4& desc) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  ptx::chain_wait();
+  ptx::chain_next();
   desc = p.desc[blockIdx.x];
   return desc.z > 0 && desc.x >= 0 && desc.x + desc.z <= kDq4MaxPieces && (desc.y & ~1) == 0;
 }

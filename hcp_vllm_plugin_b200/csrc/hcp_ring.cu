@@ -113,6 +113,23 @@ bool encode_rows_heads(CUtensorMap* m, bool f16, const void* base, int64_t rows,
   return encode_map(m, f16, 3, base, dims, strides, box);
 }
 
+// Launch as a programmatic dependent of the kernel before it in the stream: for kernels of a
+// few microseconds that begin with ptx::chain_wait().  Their scheduling overlaps that kernel's end.
+template <typename... P>
+int launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, int smem, cudaStream_t st, const P&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+  cfg.stream = st;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+}
+
 std::mutex g_attr_mu;
 bool g_attr_done[2][2][8][64];  // variants 0-6, and 7 for the LIST kernel
 bool g_dec_attr_done[2][2][64];
@@ -918,9 +935,8 @@ extern "C" int hcp_kv_plan_step(const hcp_step_plan_args* a, void* stream) {
   p.block_size = a->block_size;
   p.bs_shift = pow2_shift(a->block_size);
   const int64_t blocks = std::max<int64_t>(1, (a->num_tokens + kPlanThreads - 1) / kPlanThreads);
-  step_plan_kernel<<<static_cast<int>(std::min<int64_t>(blocks, 2 * 148)), kPlanThreads, 0,
-                     static_cast<cudaStream_t>(stream)>>>(p);
-  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+  return launch_chained(step_plan_kernel, dim3(static_cast<unsigned>(std::min<int64_t>(blocks, 2 * 148))), kPlanThreads, 0,
+                        static_cast<cudaStream_t>(stream), p);
 }
 
 namespace {
@@ -948,19 +964,14 @@ int launch_norm_rope(NormRopeParams p, int64_t tokens, int kind, cudaStream_t st
   p.kv_blocks = static_cast<unsigned>(kv_blocks);
   const unsigned blocks = static_cast<unsigned>(grid);
   auto launch = [&](auto none, auto same, auto q4) {
-    switch (kind) {
-      case HCP_ROPE_CACHE_SAME: same<<<blocks, kRopeThreads, 0, st>>>(p); break;
-      case HCP_ROPE_CACHE_Q4: q4<<<blocks, kRopeThreads, 0, st>>>(p); break;
-      default: none<<<blocks, kRopeThreads, 0, st>>>(p); break;
-    }
+    return launch_chained(kind == HCP_ROPE_CACHE_SAME ? same : kind == HCP_ROPE_CACHE_Q4 ? q4 : none, dim3(blocks),
+                          kRopeThreads, 0, st, p);
   };
   if (p.interleaved)
-    launch(norm_rope_kernel<D, F16, TAB32, kRopeCacheNone, true>, norm_rope_kernel<D, F16, TAB32, kRopeCacheSame, true>,
-           norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, true>);
-  else
-    launch(norm_rope_kernel<D, F16, TAB32, kRopeCacheNone, false>, norm_rope_kernel<D, F16, TAB32, kRopeCacheSame, false>,
-           norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, false>);
-  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+    return launch(&norm_rope_kernel<D, F16, TAB32, kRopeCacheNone, true>, &norm_rope_kernel<D, F16, TAB32, kRopeCacheSame, true>,
+                  &norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, true>);
+  return launch(&norm_rope_kernel<D, F16, TAB32, kRopeCacheNone, false>, &norm_rope_kernel<D, F16, TAB32, kRopeCacheSame, false>,
+                &norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, false>);
 }
 
 bool g_dq4_attr_done[2][2][2][64];
@@ -979,27 +990,19 @@ int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
       done = true;
     }
   }
-  decode_q4_kernel<D, F16, NT><<<kDq4Sms * dq4_ctas_per_sm(NT), kDq4Threads, smem, st>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return HCP_ERR_CUDA;
-  // the joining kernel may start while the first one ends; it waits for it itself
+  const int rc = launch_chained(decode_q4_kernel<D, F16, NT>, dim3(kDq4Sms * dq4_ctas_per_sm(NT)), kDq4Threads, smem, st, p);
+  if (rc != HCP_OK) return rc;
   const int64_t pairs = static_cast<int64_t>(p.rows) * p.num_kv_heads;
   const int64_t parts = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps / pairs + 2;  // of a pair, were the rows alike
   // From about 16 parts on they are shared between warps, 8 each; where the heads alone leave SMs
   // idle, a head's dims are split over blocks too (parts are many then).
   const bool wide = parts >= 16, split = pairs * p.group < kDq4Sms;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(pairs), wide ? static_cast<unsigned>(p.group) : 1u, split ? D / 32 : 1);
-  cfg.blockDim = dim3(32 * (wide ? static_cast<int>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8)) : std::min(p.group, 8)));
-  cfg.stream = st;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = !wide ? cudaLaunchKernelEx(&cfg, decode_q4_join_kernel<D>, p)
-                        : split ? cudaLaunchKernelEx(&cfg, decode_q4_join_wide_kernel<D, 1, 32>, p)
-                                : cudaLaunchKernelEx(&cfg, decode_q4_join_wide_kernel<D, D / 32, 8>, p);
-  return e == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+  const dim3 grid(static_cast<unsigned>(pairs), wide ? static_cast<unsigned>(p.group) : 1u, split ? D / 32 : 1);
+  const unsigned threads = 32 * (wide ? static_cast<unsigned>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8))
+                                      : static_cast<unsigned>(std::min(p.group, 8)));
+  if (!wide) return launch_chained(decode_q4_join_kernel<D>, grid, threads, 0, st, p);
+  if (split) return launch_chained(decode_q4_join_wide_kernel<D, 1, 32>, grid, threads, 0, st, p);
+  return launch_chained(decode_q4_join_wide_kernel<D, D / 32, 8>, grid, threads, 0, st, p);
 }
 
 int validate_decode_q4(const hcp_decode_q4_args* a) {
@@ -1153,14 +1156,10 @@ extern "C" int hcp_kv_cache_update_q4(const void* key, const void* value, int64_
   if (units > INT32_MAX) return HCP_ERR_UNSUPPORTED;
   const unsigned grid = static_cast<unsigned>(units);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) {
-    if (dtype == HCP_F16) q4_update_kernel<128, true><<<grid, kQ4Threads, 0, st>>>(p);
-    else q4_update_kernel<128, false><<<grid, kQ4Threads, 0, st>>>(p);
-  } else {
-    if (dtype == HCP_F16) q4_update_kernel<64, true><<<grid, kQ4Threads, 0, st>>>(p);
-    else q4_update_kernel<64, false><<<grid, kQ4Threads, 0, st>>>(p);
-  }
-  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+  const bool f16 = dtype == HCP_F16;
+  return launch_chained(head_dim == 128 ? (f16 ? q4_update_kernel<128, true> : q4_update_kernel<128, false>)
+                                        : (f16 ? q4_update_kernel<64, true> : q4_update_kernel<64, false>),
+                        dim3(grid), kQ4Threads, 0, st, p);
 }
 
 extern "C" int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, int32_t block_size,
@@ -1187,14 +1186,10 @@ extern "C" int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, 
   if (blocks > INT32_MAX) return HCP_ERR_UNSUPPORTED;
   const unsigned grid = static_cast<unsigned>(blocks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (head_dim == 128) {
-    if (dtype == HCP_F16) q4_gather_kernel<128, true><<<grid, kQ4Threads, 0, st>>>(p);
-    else q4_gather_kernel<128, false><<<grid, kQ4Threads, 0, st>>>(p);
-  } else {
-    if (dtype == HCP_F16) q4_gather_kernel<64, true><<<grid, kQ4Threads, 0, st>>>(p);
-    else q4_gather_kernel<64, false><<<grid, kQ4Threads, 0, st>>>(p);
-  }
-  return cudaGetLastError() == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+  const bool f16 = dtype == HCP_F16;
+  return launch_chained(head_dim == 128 ? (f16 ? q4_gather_kernel<128, true> : q4_gather_kernel<128, false>)
+                                        : (f16 ? q4_gather_kernel<64, true> : q4_gather_kernel<64, false>),
+                        dim3(grid), kQ4Threads, 0, st, p);
 }
 
 extern "C" int64_t hcp_decode_q4_workspace_bytes(const hcp_decode_q4_args* a) {

@@ -255,6 +255,8 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) norm_rope_kernel(co
   constexpr int kLanes = D / 8;
   constexpr int kWarpRows = 32 / kLanes;         // rows of a round
   constexpr int kAhead = 3;                      // rounds in flight
+  ptx::chain_wait();
+  ptx::chain_next();
   if constexpr (CACHE == kRopeCacheQ4) {
     __shared__ Q4Stage<D> st;
     if (blockIdx.x < p.kv_blocks) {

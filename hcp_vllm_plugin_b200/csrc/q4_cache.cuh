@@ -31,6 +31,7 @@
 #include <cstdint>
 
 #include "cache.cuh"
+#include "sm100_ptx.cuh"
 
 namespace hcp {
 
@@ -290,6 +291,8 @@ template <int D, bool F16>
 __global__ void __launch_bounds__(kQ4Threads) q4_update_kernel(const Q4UpdateParams p) {
   using L = Q4<D>;
   __shared__ Q4Stage<D> st;
+  ptx::chain_wait();
+  ptx::chain_next();
   constexpr int kRows = kQ4Threads / L::kLanes;
   const int h = blockIdx.x % p.num_kv_heads;
   long long t0;
@@ -361,6 +364,8 @@ template <int D, bool F16>
 __global__ void __launch_bounds__(kQ4Threads) q4_gather_kernel(const Q4GatherParams p) {
   using L = Q4<D>;
   constexpr int kRows = 32 / L::kLanes;  // rows of a warp's store
+  ptx::chain_wait();
+  ptx::chain_next();
   const int lane = threadIdx.x & 31;
   const long long unit = static_cast<long long>(blockIdx.x) * (kQ4Threads / 32) + threadIdx.x / 32;
   const int h = static_cast<int>(unit % p.num_kv_heads);

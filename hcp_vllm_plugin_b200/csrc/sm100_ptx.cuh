@@ -23,6 +23,14 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
   return t;
 }
 
+// ------------------------------------------------- chained launches
+// A kernel launched as a programmatic dependent may be scheduled while the one
+// before it in the stream runs out; chain_wait returns when that one has ended
+// and its writes are visible, so it stands before a kernel's first access to
+// memory.  chain_next lets the next such kernel be scheduled.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");

@@ -23,6 +23,8 @@
 #include <climits>
 #include <cstdint>
 
+#include "sm100_ptx.cuh"
+
 namespace hcp {
 
 constexpr int kPlanThreads = 256;
@@ -78,6 +80,8 @@ __global__ void __launch_bounds__(kPlanThreads) step_plan_kernel(const StepPlanP
   // starts of every thread's run of requests: tokens, new blocks
   __shared__ long long s_tok[kPlanThreads + 1], s_blk[kPlanThreads + 1];
   __shared__ long long w_tok[kPlanThreads / 32], w_blk[kPlanThreads / 32], w_want[kPlanThreads / 32];
+  ptx::chain_wait();
+  ptx::chain_next();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int run = (p.num_reqs + kPlanThreads - 1) / kPlanThreads;
   const int r0 = min(p.num_reqs, tid * run), r1 = min(p.num_reqs, r0 + run);

@@ -649,6 +649,46 @@ def test_captured_step_follows_the_lengths(ops):
         held = [a + b for a, b in zip(held, new)]
 
 
+def test_calls_wait_for_what_comes_before_them(ops):
+    """The calls may be scheduled while the kernel before them runs out: inputs written just before, by a
+    slow kernel of the same stream or of another one behind an event, are the ones they see."""
+    gen = torch.Generator().manual_seed(28)
+    cache = _filled(ops, gen, 64, 4, 16, 128, BF16)
+    table = torch.randint(0, 64, (3, 300), generator=gen, dtype=torch.int32).cuda()
+    q, lens = _randn(gen, 3, 28, 128).cuda(), _i32([4000, 17, 2500])
+    key, value = _randn(gen, 40, 4, 128).cuda(), _randn(gen, 40, 4, 128).cuda()
+    slots, pos, tab = torch.randperm(1024, generator=gen)[:40].cuda(), torch.arange(3).cuda() + 5, _angles(64, 128, torch.float32).cuda()
+    kq = _randn(gen, 3, 4, 128).cuda()
+
+    def chain(c, q_in, n, t):
+        out, lse = torch.empty_like(q), torch.empty(28, 3, device="cuda")
+        plan = ops.kv_plan_step(n, n.sign(), t, n, n[:1] * 0, block_size=16, num_tokens=3)
+        qr, _ = ops.qk_norm_rope(q_in, kq, pos, tab)
+        ops.kv_cache_update_q4(key, value, c, slots)
+        ops.decode_splitkv_q4(qr, c, t, n, scale=0.1, out=out, lse=lse)
+        k, v = ops.kv_cache_gather_q4(c, slots, BF16)
+        return out, lse, k, v, plan.kv_lens, plan.positions, t.clone()
+
+    want = chain(cache.clone(), q, lens, table.clone())
+    torch.cuda.synchronize()
+    busy = torch.randn(4096, 4096, device="cuda")
+    side = torch.cuda.Stream()
+    for other in (False, True):
+        for _ in range(3):
+            c, q_in, n, t = torch.zeros_like(cache), torch.zeros_like(q), torch.zeros_like(lens), torch.zeros_like(table)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side if other else torch.cuda.current_stream()):
+                for _ in range(4):
+                    busy = (busy @ busy).clamp(-1, 1)
+                c.copy_(cache), q_in.copy_(q), n.copy_(lens), t.copy_(table)
+            torch.cuda.current_stream().wait_stream(side)
+            got = chain(c, q_in, n, t)
+            c.zero_(), q_in.zero_(), n.zero_(), t.zero_()   # and what follows waits for them
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b)
+
+
 def test_two_captured_decodes_do_not_share_partials(ops):
     """Two graphs replayed at once on two streams, each with its own partial sums."""
     gen = torch.Generator().manual_seed(23)
