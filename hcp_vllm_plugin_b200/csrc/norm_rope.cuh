@@ -10,9 +10,9 @@
 //
 // Bound by HBM: 2 bytes read and 2 written per element.  D/8 lanes own a row and
 // each lane holds both members of its pairs (4 dims and their 4 partners), so the
-// rotation needs no exchange.  A warp takes one token: its lanes take the token's
-// cos / sin and the weights into one map and go over the token's heads, three rounds of
-// loads in flight.  With few tokens a token's rounds are spread over warps.  With the
+// rotation needs no exchange.  A warp takes one token: its lanes hold the token's
+// cos / sin and the weights and go over the token's heads, three rounds of loads in
+// flight.  With few tokens a token's rounds are spread over warps.  With the
 // 4-bit cache further blocks of the same launch take k and v, 16 tokens of one head
 // each, so that whole tiles of the cache are built in shared memory (q4_cache.cuh).
 #pragma once
@@ -106,29 +106,23 @@ __device__ __forceinline__ void rope_angles(const NormRopeParams& p, const RopeL
     rope_up4<F16>(*reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p.table) + at + p.rotary / 2), sn);
   }
 }
-// A row's map, weights and rotation in one: with u, v the members of a pair,
-//   u' = inv (u k0 - v k1), v' = inv (v k2 + u k3),  k0 = w_u cos, k1 = w_v sin, k2 = w_v cos, k3 = w_u sin,
-// inv the row's 1 / rms.  One map serves all rows of a token that share the weights.
+// What all rows of a token share that have the same weights.
 struct RopeMap {
-  float k0[4], k1[4], k2[4], k3[4];
+  float g[8], cs[4], sn[4];
 };
-template <bool F16, bool INTER>
-__device__ __forceinline__ void rope_map(RopeMap& f, const RopeLane& r, const uint16_t* w, const float* cs, const float* sn) {
-  float g[8] = {1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f, 1.f};
-  if (w != nullptr) {
-    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a0), g);
-    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a1), g + 4);
-  }
+template <bool F16>
+__device__ __forceinline__ void rope_weights(RopeMap& f, const RopeLane& r, const uint16_t* w) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float gu = INTER ? g[2 * i] : g[i], gv = INTER ? g[2 * i + 1] : g[4 + i];
-    f.k0[i] = gu * cs[i];
-    f.k1[i] = gv * sn[i];
-    f.k2[i] = gv * cs[i];
-    f.k3[i] = gu * sn[i];
+  for (int i = 0; i < 8; ++i) f.g[i] = 1.f;
+  if (w != nullptr) {
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a0), f.g);
+    rope_up4<F16>(*reinterpret_cast<const uint2*>(w + r.a1), f.g + 4);
   }
 }
-// Norm and rotation of one row; every lane of the warp takes part.
+// Norm and rotation of one row; every lane of the warp takes part.  The products are rounded
+// as the formula has them: (x inv) w, then u cos - v sin.  Weights, angles and inv in one map
+// would save a third of the multiplications (51 against 54 us at 16384 tokens) and round five
+// times as many keys to the other neighbour, each of which may turn a step of the 4-bit cache.
 template <int D, bool F16, bool INTER>
 __device__ __forceinline__ void rope_row(const RopeLane& r, const RopeMap& f, bool norm, float eps, const uint2 (&in)[2],
                                          uint2 (&out)[2]) {
@@ -140,18 +134,21 @@ __device__ __forceinline__ void rope_row(const RopeLane& r, const RopeMap& f, bo
   for (int i = 0; i < 8; ++i) sq = fmaf(x[i], x[i], sq);
 #pragma unroll
   for (int s = 1; s < D / 8; s <<= 1) sq += __shfl_xor_sync(0xffffffffu, sq, s);
-  const float inv = norm ? rsqrtf(fmaf(sq, 1.f / D, eps)) : 1.f;
+  if (norm) {
+    const float inv = rsqrtf(fmaf(sq, 1.f / D, eps));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int a = INTER ? 2 * i : i, b = INTER ? 2 * i + 1 : i + 4;
-    y[a] = x[a] * f.k0[i];
-    y[b] = x[b] * f.k2[i];
-    if (r.turns) {  // (the other dims meet no sine: an infinity would not stay in its place)
-      y[a] = fmaf(-x[b], f.k1[i], y[a]);
-      y[b] = fmaf(x[a], f.k3[i], y[b]);
+    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inv), f.g[i]);
+  }
+  if (r.turns) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int a = INTER ? 2 * i : i, b = INTER ? 2 * i + 1 : i + 4;
+      y[a] = __fsub_rn(__fmul_rn(x[a], f.cs[i]), __fmul_rn(x[b], f.sn[i]));
+      y[b] = __fadd_rn(__fmul_rn(x[b], f.cs[i]), __fmul_rn(x[a], f.sn[i]));
     }
-    y[a] *= inv;
-    y[b] *= inv;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
   }
   out[0] = rope_down4<F16>(y);
   out[1] = rope_down4<F16>(y + 4);
@@ -193,11 +190,10 @@ __device__ __forceinline__ void rope_kv_block(const NormRopeParams& p, int unit,
       in[1] = *reinterpret_cast<const uint2*>(k + ln.a1);
       vraw = reinterpret_cast<const uint4*>(p.v + tok * p.v_stride + static_cast<long long>(h) * D)[c];
     }
-    float cs[4], sn[4];
-    rope_angles<F16, TAB32>(p, ln, pos, c, cs, sn);
-    if (pos >= p.table_rows) in[0] = in[1] = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN
     RopeMap f;
-    rope_map<F16, INTER>(f, ln, p.k_weight, cs, sn);
+    rope_angles<F16, TAB32>(p, ln, pos, c, f.cs, f.sn);
+    if (pos >= p.table_rows) in[0] = in[1] = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN
+    rope_weights<F16>(f, ln, p.k_weight);
     rope_row<D, F16, INTER>(ln, f, p.k_weight != nullptr, p.eps, in, out);
     if (pos >= 0) {
       uint16_t* k = p.k_out + tok * p.k_out_stride + static_cast<long long>(h) * D;
@@ -299,15 +295,11 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) norm_rope_kernel(co
   }
   uint16_t* const qo = p.q_out + tok * p.q_out_stride;
   uint16_t* const ko = p.k_out + tok * p.k_out_stride - static_cast<long long>(H) * D;
-  bool keys = begin + sub >= H;                  // rows rise: queries' map, then keys'
+  bool keys = begin + sub >= H;                  // rows rise: queries, then keys
   bool norm = (keys ? p.k_weight : p.q_weight) != nullptr;
   RopeMap f;
-  auto map = [&](const uint16_t* w) {  // (the angles again for the keys: kept, they would cost 8 registers)
-    float cs[4], sn[4];
-    rope_angles<F16, TAB32>(p, ln, pos, c, cs, sn);
-    rope_map<F16, INTER>(f, ln, w, cs, sn);
-  };
-  map(keys ? p.k_weight : p.q_weight);
+  rope_angles<F16, TAB32>(p, ln, pos, c, f.cs, f.sn);
+  rope_weights<F16>(f, ln, keys ? p.k_weight : p.q_weight);
   for (int r0 = begin; r0 < end; r0 += kAhead * kWarpRows) {
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
@@ -316,7 +308,7 @@ __global__ void __launch_bounds__(kRopeThreads, kRopeBlocks) norm_rope_kernel(co
       if (CACHE != kRopeCacheQ4 && !keys && r >= H) {
         keys = true;
         norm = p.k_weight != nullptr;
-        map(p.k_weight);
+        rope_weights<F16>(f, ln, p.k_weight);
       }
       if (!known) in[i][0] = in[i][1] = make_uint2(0x7fff7fffu, 0x7fff7fffu);  // NaN
       rope_row<D, F16, INTER>(ln, f, norm, p.eps, in[i], out);
