@@ -35,6 +35,12 @@
 // to out from the warp's registers; one that is cut leaves a partial (O, base, sum)
 // per piece in the workspace, and a second kernel, already resident when the first
 // ends, joins them in order.
+//
+// Measured (28 heads over 4, D 128, bf16; a replayed graph): 64 rows x 32768 keys 234 us =
+// 5.2 TB/s, 0.80 of the measured copy rate, with 288 instructions a tile on three warps a
+// scheduler as the bound (250 us with every page in L2 as well); 1 x 131072 keys 26 us; 16 rows of
+// up to 300 keys 11.6 us, latencies.  Four warps a scheduler leave 128 registers, too few for
+// two tiles a step (254 us); two leave latency (255 us).
 #pragma once
 
 #include <cuda_bf16.h>

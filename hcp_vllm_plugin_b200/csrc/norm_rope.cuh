@@ -15,6 +15,9 @@
 // flight.  With few tokens a token's rounds are spread over warps.  With the
 // 4-bit cache further blocks of the same launch take k and v, 16 tokens of one head
 // each, so that whole tiles of the cache are built in shared memory (q4_cache.cuh).
+//
+// Measured at 16384 tokens of 28/4 heads, D 128, bf16: 54 us (277 MB, 5.1 TB/s, 0.79 of the
+// measured copy rate), 62 us with the 16-bit cache, 67 us with the 4-bit one.
 #pragma once
 
 #include <cuda_bf16.h>

@@ -286,7 +286,9 @@ __device__ __forceinline__ void q4_flush(const Q4Stage<D>& st, uint8_t* cache) {
 
 // A block takes 16 tokens of one head: D/8 lanes a row quantise K and V rows into the
 // staged tile, which leaves in 16-byte pieces where it is whole (a chunk of a prefill),
-// token by token elsewhere (decodes).  Bound by HBM: 2 bytes read, 9/16 written an element.
+// token by token elsewhere (decodes).  HBM's share is 2 bytes read, 9/16 written an element; what
+// bounds it is the quantisation's instructions (77% of the issue slots): 13.3 us for 16384 rows of 4
+// heads, D 128, against 6.7 us of bytes; 45 us with byte stores straight to the cache.
 template <int D, bool F16>
 __global__ void __launch_bounds__(kQ4Threads) q4_update_kernel(const Q4UpdateParams p) {
   using L = Q4<D>;
@@ -359,7 +361,8 @@ __device__ __forceinline__ uint4 q4_open8(uint32_t w, uint32_t sm) {
 
 // A warp takes a run of 16 tokens of one head (runs as in the scatter).  Where the run is a
 // whole tile, V is read in its 16-byte pieces of 4 tokens x 8 dims; rows leave in full lines
-// either way.  Bound by HBM: 9/16 bytes read, 2 written an element.
+// either way.  Bound by HBM: 9/16 bytes read, 2 written an element.  Measured: 7.8 us for 16384
+// rows of 4 heads, D 128 (15.6 us token by token).
 template <int D, bool F16>
 __global__ void __launch_bounds__(kQ4Threads) q4_gather_kernel(const Q4GatherParams p) {
   using L = Q4<D>;

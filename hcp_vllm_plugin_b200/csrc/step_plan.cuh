@@ -17,7 +17,9 @@
 // of consecutive requests, then one scan of 256 pairs) and works on its share
 // of the tokens and of the new table entries.  A token that falls into a new
 // block reads its id from the free list and not from the table, which another
-// block may be writing; the entries below have_i are only read.
+// block may be writing; the entries below have_i are only read.  Measured: 2.7 us for
+// 8 requests, 4.7 us for 1024 (7.0 with 64-bit divisions by the block size), 4.0 us for 257
+// requests with 20000 token rows.
 #pragma once
 
 #include <climits>
