@@ -13,19 +13,19 @@
 //       o_g    = sum_j (p_j s_j) (n_j - 8)     + sum_j p_j (lo_j + 8 s_j)
 //     V is centred, so that sums over many keys stay as small as their own terms; a
 //     score's sum is over 64 products, where the offset costs 6 bits of 24 and saves
-//     the centring (a seventh of the kernel's instructions);
+//     the centring (a ninth of the kernel's instructions);
 //   * keys are the rows of the first product (16 keys x 8 heads) and dims those of
 //     the second (16 dims x 8 heads), so a group of up to 8 query heads fills the
 //     instruction's 8 columns instead of half of 16 rows;
 //   * the tile layout gives every lane its fragments of both products in whole
-//     16-byte pieces: no shared memory, no transposes; only the 8 x 8 blocks of P
-//     are transposed between the products (movmatrix);
+//     16-byte pieces: no transposes but of the 8 x 8 blocks of P between the products
+//     (movmatrix);
 //   * q and p_j s_j enter the products in fp16, scaled by powers of two: q by its
 //     head's largest element (no loss), p_j s_j by the largest scale met so far.
 //     Rounding p_j s_j to 11 bits is off by at most 2^-11 of each key's term, and the
-//     terms' weights sum to one: a quarter of what rounding the result to bf16 may be
-//     off.  A second product for the rest costs 8 of the 16 matrix instructions and
-//     a tenth of the issue slots of a kernel that is bound by them.
+//     terms' weights sum to one: an eighth of what rounding the result to bf16 may be
+//     off.  A second product for the rest would add 8 matrix instructions to a tile's 16
+//     and a tenth to the issue slots of a kernel that is bound by them.
 //
 // Split: all rows' tiles of 16 keys, heads outermost in a row, form one line that
 // the warps cut into equal pieces, so any mix of lengths is even and nothing about
@@ -33,8 +33,8 @@
 // warp works alone: its tiles come through a ring of asynchronous copies in shared
 // memory, two tiles a step.  A (row, KV head) that lies inside one piece is written
 // to out from the warp's registers; one that is cut leaves a partial (O, base, sum)
-// per piece in the workspace, and a second kernel, already resident when the first
-// ends, joins them in order.
+// per piece in the workspace, and a second kernel, scheduled as the first runs out,
+// joins them in order.
 //
 // Measured (28 heads over 4, D 128, bf16; a replayed graph): 64 rows x 32768 keys 234 us =
 // 5.2 TB/s, 0.80 of the measured copy rate, with 288 instructions a tile on three warps a
@@ -336,8 +336,9 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     for (int i = 0; i < kDq4Stages - 1; ++i) issue(i);
 
     // ---- Q fragments: columns are heads, lane's k index pairs (d, d + 4).  Each head is
-    // scaled by a power of two to the top of fp16's range and rounded to it: exact down to
-    // 2^-29 of its largest element for 11-bit elements.  The power goes into the head's factor.
+    // scaled by a power of two into fp16's range and rounded to it: exact but for elements below
+    // 2^-18 of its largest, which are off by at most 2^-29 of that.  (Not to the range's top: sums
+    // times large scales have to stay finite.)  The power goes into the head's factor.
     uint32_t qb[NT][2 * KW][2];
     float sq[NT][NG][2];  // 16 times the sums of the scaled q over each group, heads 2t and 2t+1
     float hs[NT][2];      // score in log2 units = hs * 16 (scaled q . k)
@@ -353,9 +354,9 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e with top * 2^e in [2^14, 2^15), e at most 126 (and 0 for an empty or infinite head)
+      // 2^e with top * 2^e in [2^4, 2^5), e at most 126 (and 0 for an empty or infinite head)
       const int ex = static_cast<int>(__float_as_uint(top) >> 23);
-      const int e = ex == 0 || ex == 255 ? 0 : min(126, 141 - ex);
+      const int e = ex == 0 || ex == 255 ? 0 : min(126, 131 - ex);
       const float up = __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
       float part[NG];
 #pragma unroll
@@ -569,8 +570,9 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
         for (int nt = 0; nt < NT; ++nt) {
           // pairs of heads in packed arithmetic
           const float2 f = make_float2(hs[nt][0], hs[nt][1]), b = make_float2(-base[nt][0], -base[nt][1]);
-          const float2 x0 = __ffma2_rn(make_float2(sc[u][nt][0], sc[u][nt][1]), f, b);
-          const float2 x1 = __ffma2_rn(make_float2(sc[u][nt][2], sc[u][nt][3]), f, b);
+          // (the product rounded as in the base: the largest score's weight is 1 however large it is)
+          const float2 x0 = __fadd2_rn(__fmul2_rn(make_float2(sc[u][nt][0], sc[u][nt][1]), f), b);
+          const float2 x1 = __fadd2_rn(__fmul2_rn(make_float2(sc[u][nt][2], sc[u][nt][3]), f), b);
           pr[u][nt][0] = ex2_approx(x0.x);
           pr[u][nt][1] = ex2_approx(x0.y);
           pr[u][nt][2] = ex2_approx(x1.x);

@@ -470,6 +470,10 @@ def test_decode_q4_scales_far_apart(ops, dtype):
     q = (torch.randn(3, h, d, generator=gen) * 10.0 ** torch.linspace(-4, 1, h)[:, None]).to(dtype)
     table = torch.arange(nb, dtype=torch.int32).view(1, nb).repeat(3, 1)
     _run_decode(ops, cache, q, [n, 200, 45], table, dtype)
+    # scores up to 10^6: the largest key takes all, and everything stays finite
+    ops.kv_cache_update_q4((torch.randn(n, hkv, d, generator=gen) * 300).to(dtype).cuda(), v.to(dtype).cuda(), cache,
+                           torch.arange(n, device="cuda"))
+    _run_decode(ops, cache, (torch.randn(3, h, d, generator=gen) * 300).to(dtype), [n, 200, 45], table, dtype)
     # far past fp16's range either way, in bf16 (64 bits do not pass 10^38 either)
     if dtype == BF16:
         for size in (1e-30, 1e30):
@@ -477,6 +481,9 @@ def test_decode_q4_scales_far_apart(ops, dtype):
                                    torch.arange(n, device="cuda"))
             _run_decode(ops, cache, _randn(gen, 3, h, d), [n, 200, 45], table, dtype)
             _run_decode(ops, cache, (torch.randn(3, h, d, generator=gen) * 1e-20).to(dtype), [n, 200, 45], table, dtype)
+            ops.kv_cache_update_q4((torch.randn(n, hkv, d, generator=gen) * size).to(dtype).cuda(), v.to(dtype).cuda(), cache,
+                                   torch.arange(n, device="cuda"))
+            _run_decode(ops, cache, (torch.randn(3, h, d, generator=gen) / size).to(dtype), [n, 200, 45], table, dtype)
 
 
 def test_decode_q4_strided_rows_and_own_workspace(ops):
