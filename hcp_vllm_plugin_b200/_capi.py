@@ -258,6 +258,8 @@ def front():
     if _front is None:
         lib = load()
         try:
+            import torch  # noqa: F401 - brings the libraries that the module links
+
             from . import _hcp_front as mod
         except ImportError as e:
             raise HcpError(f"_hcp_front.so cannot be loaded ({e}): build it for this torch with "
