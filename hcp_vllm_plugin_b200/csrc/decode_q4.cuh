@@ -21,11 +21,14 @@
 //     16-byte pieces: no transposes but of the 8 x 8 blocks of P between the products
 //     (movmatrix);
 //   * q and p_j s_j enter the products in fp16, scaled by powers of two: q by its
-//     head's largest element (no loss), p_j s_j by the largest scale met so far.
-//     Rounding p_j s_j to 11 bits is off by at most 2^-11 of each key's term, and the
-//     terms' weights sum to one: an eighth of what rounding the result to bf16 may be
-//     off.  A second product for the rest would add 8 matrix instructions to a tile's 16
-//     and a tenth to the issue slots of a kernel that is bound by them.
+//     head's largest element (no loss), p_j s_j by the largest of them that the head
+//     and group met so far, in weights of the present base: a scale counts by what its
+//     key weighs, so a large value that nobody attends takes no bits from the others.
+//     Rounding p_j s_j to 11 bits is off by at most 2^-11 of each key's term, and by
+//     2^-33 of the largest p s where that is more (fp16's smallest numbers).  The terms'
+//     weights sum to one: an eighth of what rounding the result to bf16 may be off, as
+//     much as rounding it to fp16.  A second product for the rest would add 8 matrix
+//     instructions to a tile's 16.
 //
 // Split: all rows' tiles of 16 keys, heads outermost in a row, form one line that
 // the warps cut into equal pieces, so any mix of lengths is even and nothing about
@@ -59,6 +62,7 @@ constexpr int kDq4MaxPieces = kDq4MaxCtas * kDq4Warps;
 constexpr int kDq4Stages = 3;    // steps of a warp's ring: one read, the others in flight
 constexpr int kDq4Step = 2;      // tiles of a step, and of a piece at least
 constexpr int kDq4JoinWarps = 16;
+constexpr int kDq4UnitTop = 127 + 118;  // exponent of the finest unit's reciprocal: p_j <= 2^8 times it stays finite
 // Blocks of an SM: 168 registers a thread, and twice the sums beyond 8 heads a group.
 constexpr int dq4_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
@@ -137,6 +141,12 @@ __device__ __forceinline__ void q4_pairs(uint32_t w, const Q4Consts& c, uint32_t
     asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[2 * i]) : "r"(a), "r"(0xe408e408u));     // - 1032
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r[2 * i + 1]) : "r"(b), "r"(0x2c002c00u), "r"(c.k72));  // / 16 - 72
   }
+}
+
+__device__ __forceinline__ uint32_t q4_max2_f16(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // The same pairs as 1024 + 16 n, without the centring: for products whose sums start
@@ -390,19 +400,13 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     float vz[NT][NG][2], l_run[NT][2];
     float base[NT][2];   // of the weights: the running maximum or up to 8 below it; 0 before the first key
     float limit[NT][2];  // the score at which the base has to rise: (base + 8) / hs, -inf before the first key
-    float vref[NG];      // powers of two: the sums o are in units of vref, 1 / vref multiplies V's scales
-    float vinv[NG], vlim[NG];
-#pragma unroll
-    for (int a = 0; a < NG; ++a) {
-      vref[a] = 0.f;
-      vinv[a] = 0.f;
-      vlim[a] = 0.f;
-    }
+    float vinv[NT][NG][2];  // powers of two that multiply p_j s_j: the sums o are in units of 1 / vinv
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int a = 0; a < NG; ++a) {
         vz[nt][a][0] = vz[nt][a][1] = 0.f;
+        vinv[nt][a][0] = vinv[nt][a][1] = __uint_as_float(kDq4UnitTop << 23);
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][a][i][0] = o[nt][a][i][1] = o[nt][a][i][2] = o[nt][a][i][3] = 0.f;
       }
@@ -500,17 +504,11 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
       }
       float vs[U][2][NG];
 #pragma unroll
-      for (int a = 0; a < NG; ++a) {
-        float mx = 0.f;
+      for (int a = 0; a < NG; ++a)
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            vs[u][e][a] = q4_up<F16>(prm[u][e][NG + a] & 0xffffu);
-            mx = fmaxf(mx, vs[u][e][a]);
-          }
-        raise = raise || mx > vlim[a];
-      }
+          for (int e = 0; e < 2; ++e) vs[u][e][a] = q4_up<F16>(prm[u][e][NG + a] & 0xffffu);
       if (__any_sync(0xffffffffu, raise)) {
         // a score above the base by more than 8 raises it (weights <= 2^8)
 #pragma unroll
@@ -528,40 +526,21 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
             base[nt][e] = now == -INFINITY ? 0.f : now;
             limit[nt][e] = now == -INFINITY ? -INFINITY : __fdividef(now + kRescaleThreshold, hs[nt][e]);
             l_run[nt][e] *= al;
+            const int ea = static_cast<int>(__float_as_uint(al) >> 23);
 #pragma unroll
             for (int a = 0; a < NG; ++a) {
               vz[nt][a][e] *= al;
+              // the unit falls with the weights it stands for, by al's power of two; the rest of al is the sums'
+              const int ev = static_cast<int>(__float_as_uint(vinv[nt][a][e]) >> 23), to = max(1, min(ev + 127 - ea, kDq4UnitTop));
+              const float f = ea == 0 ? 0.f : __uint_as_float(__float_as_uint(al) + (static_cast<uint32_t>(to - ev) << 23));
+              vinv[nt][a][e] = __uint_as_float(static_cast<uint32_t>(to) << 23);
 #pragma unroll
               for (int i2 = 0; i2 < 4; ++i2) {
-                o[nt][a][i2][e] *= al;
-                o[nt][a][i2][e + 2] *= al;
+                o[nt][a][i2][e] *= f;
+                o[nt][a][i2][e + 2] *= f;
               }
             }
           }
-        // a scale above 2^7 vref raises vref: weight times scale stays below 2^15 in fp16
-#pragma unroll
-        for (int a = 0; a < NG; ++a) {
-          float mx = 0.f;
-#pragma unroll
-          for (int u = 0; u < U; ++u) mx = fmaxf(mx, fmaxf(vs[u][0][a], vs[u][1][a]));
-#pragma unroll
-          for (int s = 4; s < 32; s <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, s));
-          if (mx > vlim[a]) {
-            // 2^6 vref <= mx < 2^7 vref now (vref and 1 / vref stay normal numbers)
-            const int ex = max(static_cast<int>(__float_as_uint(mx) >> 23) - 6, 1);
-            const float now = __uint_as_float(static_cast<uint32_t>(ex) << 23);
-            vinv[a] = __uint_as_float(static_cast<uint32_t>(254 - ex) << 23);
-            const float al = vref[a] * vinv[a];
-            vref[a] = now;
-            vlim[a] = now * 128.f;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int i2 = 0; i2 < 4; ++i2)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[nt][a][i2][e] *= al;
-          }
-        }
       }
       float pr[U][NT][4];
 #pragma unroll
@@ -582,6 +561,61 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
           l_run[nt][0] = l.x;
           l_run[nt][1] = l.y;
         }
+      // ---- the weights of the second product, p_j s_j in units of 1 / vinv
+      uint32_t bp[U][NT][NG][2];
+      uint32_t largest;
+      auto weigh = [&] {
+        largest = 0u;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int a = 0; a < NG; ++a) {
+              const float2 unit = make_float2(vinv[nt][a][0], vinv[nt][a][1]);
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float2 y = __fmul2_rn(__fmul2_rn(make_float2(pr[u][nt][2 * e], pr[u][nt][2 * e + 1]), unit),
+                                            make_float2(vs[u][e][a], vs[u][e][a]));
+                bp[u][nt][a][e] = pack2<true>(y.x, y.y);
+                largest = q4_max2_f16(largest, bp[u][nt][a][e]);
+              }
+            }
+      };
+      weigh();
+      // one at 2^15 or above raises its head's and group's unit, so that the largest is in [2^8, 2^9)
+      if (__any_sync(0xffffffffu, ((largest + 0x08000800u) & 0x80008000u) != 0u)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int a = 0; a < NG; ++a) {
+            uint32_t top = 0u;  // exponents of 2^-16 times the largest, of both heads (p is at most 2^8, a scale 2^124)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = 0.f;
+#pragma unroll
+              for (int u = 0; u < U; ++u)
+                mx = fmaxf(mx, fmaxf(pr[u][nt][e] * (vs[u][0][a] * 0x1p-16f), pr[u][nt][e + 2] * (vs[u][1][a] * 0x1p-16f)));
+              top |= (__float_as_uint(mx) >> 23) << (16 * e);
+            }
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int em = static_cast<int>(e == 0 ? top & 0xffffu : top >> 16);
+              const int ev = static_cast<int>(__float_as_uint(vinv[nt][a][e]) >> 23);
+              const int to = em + ev >= 253 ? max(246 - em, 1) : ev;  // (2^16 mx vinv >= 2^15)
+              const float f = __uint_as_float(static_cast<uint32_t>(max(127 + to - ev, 0)) << 23);
+              vinv[nt][a][e] = __uint_as_float(static_cast<uint32_t>(to) << 23);
+#pragma unroll
+              for (int i2 = 0; i2 < 4; ++i2) {
+                o[nt][a][i2][e] *= f;
+                o[nt][a][i2][e + 2] *= f;
+              }
+            }
+          }
+        weigh();
+      }
       // ---- O += V^T P per group
 #pragma unroll
       for (int a = 0; a < NG; ++a)
@@ -591,24 +625,21 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
           const uint32_t vwords[4] = {vw.x, vw.y, vw.z, vw.w};
           const float z0 = fmaf(8.f, vs[u][0][a], q4_up<F16>(prm[u][0][NG + a] >> 16));
           const float z1 = fmaf(8.f, vs[u][1][a], q4_up<F16>(prm[u][1][NG + a] >> 16));
-          const float s0 = vs[u][0][a] * vinv[a], s1 = vs[u][1][a] * vinv[a];
-          uint32_t bp[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             const float2 p0 = make_float2(pr[u][nt][0], pr[u][nt][1]), p1 = make_float2(pr[u][nt][2], pr[u][nt][3]);
             const float2 zv = __ffma2_rn(p0, make_float2(z0, z0), __ffma2_rn(p1, make_float2(z1, z1), make_float2(vz[nt][a][0], vz[nt][a][1])));
             vz[nt][a][0] = zv.x;
             vz[nt][a][1] = zv.y;
-            const float2 y0 = __fmul2_rn(p0, make_float2(s0, s0)), y1 = __fmul2_rn(p1, make_float2(s1, s1));
-            bp[nt][0] = movmatrix_t(pack2<true>(y0.x, y0.y));
-            bp[nt][1] = movmatrix_t(pack2<true>(y1.x, y1.y));
+            bp[u][nt][a][0] = movmatrix_t(bp[u][nt][a][0]);
+            bp[u][nt][a][1] = movmatrix_t(bp[u][nt][a][1]);
           }
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
             uint32_t fa[4];  // dims 2p (row g) and 2p+1 (row g+8) of tokens 4t, 4t+2 and 4t+1, 4t+3
             q4_pairs(vwords[i2], consts, fa);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][a][i2], fa, bp[nt][0], bp[nt][1]);
+            for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][a][i2], fa, bp[u][nt][a][0], bp[u][nt][a][1]);
           }
         }
     }
@@ -640,10 +671,11 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
 #pragma unroll
         for (int a = 0; a < NG; ++a) {
           float v[8];
+          const float unit = __uint_as_float((254u << 23) - __float_as_uint(vinv[nt][a][e]));  // 1 / vinv
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
-            v[2 * i2] = fmaf(o[nt][a][i2][e], vref[a], vz[nt][a][e]) * inv;
-            v[2 * i2 + 1] = fmaf(o[nt][a][i2][e + 2], vref[a], vz[nt][a][e]) * inv;
+            v[2 * i2] = fmaf(o[nt][a][i2][e], unit, vz[nt][a][e]) * inv;
+            v[2 * i2 + 1] = fmaf(o[nt][a][i2][e + 2], unit, vz[nt][a][e]) * inv;
           }
           const int d = 8 * (8 * a + g);
           if (whole) {

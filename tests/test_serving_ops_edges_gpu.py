@@ -1,0 +1,89 @@
+"""GPU tests of the serving-step operators where single calls went wrong or could:
+values of very different sizes, neighbours in a stream, calls that fail, captures."""
+
+import numpy as np
+import pytest
+import torch
+
+import serving_ref as R
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16 = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from hcp_vllm_plugin_b200 import _capi, ops
+    _capi.load()
+    yield ops
+    assert _capi.device_status() == 0
+
+
+def _i32(x):
+    return torch.tensor(np.asarray(x, np.int32), device="cuda")
+
+
+# ------------------------------------------------------------------ values of very different sizes
+
+def _check_by_weight(got, lse, q, k, v, scale, dtype, what):
+    """One row against 64 bits, each key's share of the bar in proportion to its own weight.
+
+    With p_j the softmax weights and top_j the largest |v| of key j's 64 dims: a score is off by at most
+    dx = 2^-17 scale sum_d |q_d| max_j |k_jd| (64 products summed in 32 bits per group, then the groups),
+    which moves the result by at most (e^(2 dx) - 1) sum p_j top_j; ex2 by 2^-21, and 2^-15 covers it and the
+    normalisation.  p_j s_j is rounded to 11 bits, off by 2^-11 p_j s_j |n_j - 8|, where 8 s_j <= 1.08 top_j
+    (15 s_j is the range, at most 2 top_j, rounded by 2^-8); below fp16's normal numbers it is off by 2^-25 of
+    a unit that is at most 2^-8 of the largest p s, so by 8 n 2^-33 max p_j s_j <= n 2^-32 sum p_j top_j in all.
+    Each of a tile's sums rounds by 2^-23 of what is summed, n / 16 tiles of them twice."""
+    n, group = k.shape[0], q.shape[0] // k.shape[1]
+    for i in range(q.shape[0]):
+        kh, vh = k[:, i // group], v[:, i // group]
+        x = kh @ q[i] * scale
+        m = x.max()
+        p = np.exp(x - m)
+        total = p.sum()
+        o = p @ vh / total
+        top = np.repeat(np.abs(vh).reshape(n, -1, 64).max(-1), 64, axis=1)
+        held = p @ top / total
+        dx = 2.0 ** -17 * scale * (np.abs(q[i]) * np.abs(kh).max(0)).sum()
+        slack = held * (np.expm1(2 * dx) + 1.08 * 2.0 ** -11 + 2.0 ** -15 + n / 8 * 2.0 ** -23 + n * 2.0 ** -32)
+        eps = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
+        bar = slack + eps * (np.abs(o) + slack) + (2.0 ** -25 if dtype == F16 else 0.0)
+        assert (np.abs(got[i] - o) <= bar).all(), (what, i, np.max(np.abs(got[i] - o) / bar))
+        ref = m + np.log(total)
+        assert abs(lse[i] - ref) <= dx + 2.0 ** -20 * (abs(ref) + 1) + n / 16 * 2.0 ** -24, (what, i)
+
+
+@pytest.mark.parametrize("h,hkv,d,dtype", [(28, 4, 128, BF16), (14, 2, 64, F16), (32, 2, 128, BF16), (12, 1, 64, BF16)])
+@pytest.mark.parametrize("case", ["first", "inside", "no weight", "falling"])
+def test_decode_q4_large_values_without_weight(ops, case, h, hkv, d, dtype):
+    """A value far larger than the others whose key has next to no weight, or had one until a better key came,
+    costs the others nothing.  Rows are many, so that one warp passes over many tiles of a row."""
+    gen = torch.Generator().manual_seed(h + d)
+    rows, bs, nb = 48, 16, 60
+    n = nb * bs - 5
+    small, large = (2.0 ** -14, 2.0 ** 14) if dtype == F16 else (1.0, 2.0 ** 34)
+    k, v = torch.randn(n, hkv, d, generator=gen), torch.randn(n, hkv, d, generator=gen)
+    q = 1 + 0.25 * torch.randn(rows, h, d, generator=gen)
+    if case == "falling":   # scores rise from -40 to 0 while values fall
+        line = torch.linspace(0, 1, n)[:, None, None]
+        k = 0.25 * k - (1 - line) * 40 / d ** 0.5
+        v = v * small * (large / small) ** (1 - line)
+    else:
+        at = [0] if case == "first" else [5, 400, 401, n - 1]
+        v *= small
+        for j in at:
+            k[j] = -(200.0 if case == "no weight" else 45.0) / d ** 0.5
+            v[j] *= large / small
+    k, v, q = k.to(dtype), v.to(dtype), q.to(dtype)
+    cache = torch.zeros(ops.kv_cache_q4_shape(nb, hkv, bs, d), dtype=torch.uint8, device="cuda")
+    ops.kv_cache_update_q4(k.cuda(), v.cuda(), cache, torch.arange(n, device="cuda"))
+    kq, vq = R.read_q4(cache.cpu().numpy(), np.arange(n), dtype)
+    table, lens, req = torch.arange(nb, dtype=torch.int32, device="cuda").view(1, nb), _i32([n] * rows), _i32([0] * rows)
+    for kind in (dtype, torch.float32):
+        out, lse = torch.zeros(rows, h, d, dtype=kind, device="cuda"), torch.zeros(h, rows, device="cuda")
+        ops.decode_splitkv_q4(q.cuda(), cache, table, lens, scale=d ** -0.5, out=out, lse=lse, token_req=req)
+        o, l = R.f64(out), R.f64(lse)
+        for r in range(0, rows, 7):
+            _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq, vq, d ** -0.5, kind, (case, r))
