@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     // page of tile 32 b + lane; the next 32 are on their way while these are used
     auto pages = [&](int b) {
       int v = -1;
-      if (32 * b + lane < n) v = __ldg(bt + ((t0 + 32 * b + lane) >> p.sub_shift));
+      if (32 * b + lane < n) v = bt[(t0 + 32 * b + lane) >> p.sub_shift];
       return v;  // looked at when it is used
     };
     int page = pages(0), page_next = pages(1);

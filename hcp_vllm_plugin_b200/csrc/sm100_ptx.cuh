@@ -27,7 +27,9 @@ __device__ __forceinline__ uint64_t global_timer_ns() {
 // A kernel launched as a programmatic dependent may be scheduled while the one
 // before it in the stream runs out; chain_wait returns when that one has ended
 // and its writes are visible, so it stands before a kernel's first access to
-// memory.  chain_next lets the next such kernel be scheduled.
+// memory.  chain_next lets the next such kernel be scheduled.  What the stream wrote
+// is read by ordinary loads: the read-only path (__ldg) asks for data that nobody
+// writes while the kernel lives, and it lives before chain_wait.
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

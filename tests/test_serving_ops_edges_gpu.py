@@ -87,3 +87,36 @@ def test_decode_q4_large_values_without_weight(ops, case, h, hkv, d, dtype):
         o, l = R.f64(out), R.f64(lse)
         for r in range(0, rows, 7):
             _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq, vq, d ** -0.5, kind, (case, r))
+
+
+# ------------------------------------------------------------------ neighbours in a stream
+
+def test_decode_right_after_the_plan_sees_its_pages(ops):
+    """Attention as the kernel right behind the plan, over a table whose new entries stand beside old ones."""
+    gen = torch.Generator().manual_seed(30)
+    reqs, width, h, hkv, d, bs = 200, 24, 28, 4, 128, 16
+    nb = reqs * width
+    cache = torch.zeros(ops.kv_cache_q4_shape(nb, hkv, bs, d), dtype=torch.uint8, device="cuda")
+    rows = torch.randn(4096, hkv, d, generator=gen).to(BF16).cuda()
+    for at in range(0, nb * bs, 4096):
+        n = min(4096, nb * bs - at)
+        ops.kv_cache_update_q4(rows[:n], rows[:n].flip(0), cache, torch.arange(at, at + n, device="cuda"))
+    q, free = torch.randn(reqs, h, d, generator=gen).to(BF16).cuda(), torch.randperm(nb, generator=gen).int().cuda()
+    head = torch.zeros(1, dtype=torch.int32, device="cuda")
+    table = torch.full((reqs, width), -1, dtype=torch.int32, device="cuda")
+    held, outs, wants = np.zeros(reqs, np.int64), [], []
+    for step in range(12):
+        new = torch.randint(0, 33, (reqs,), generator=gen).numpy()
+        ctx, add = _i32(held), _i32(new)
+        out = torch.zeros_like(q)
+        torch.cuda.synchronize()
+        plan = ops.kv_plan_step(ctx, add, table, free, head, block_size=bs, num_tokens=reqs)
+        ops.decode_splitkv_q4(q, cache, table, plan.seq_lens, scale=d ** -0.5, out=out)
+        torch.cuda.synchronize()
+        want = torch.zeros_like(q)
+        ops.decode_splitkv_q4(q, cache, table.clone(), plan.seq_lens.clone(), scale=d ** -0.5, out=want)
+        outs.append(out), wants.append(want)
+        held, head = held + new, plan.free_head.clone()
+        assert plan.missing.item() == 0
+    for a, b in zip(outs, wants):
+        assert torch.equal(a, b)
