@@ -895,6 +895,49 @@ extern "C" int hcp_kv_cache_gather(const void* kv_cache, int64_t num_blocks, int
 // A serving step's data path beside the attention kernels: cache plan, norm and
 // rotation, the 4-bit cache and attention over it.
 // ---------------------------------------------------------------------------
+namespace {
+
+// A buffer of `rows` pieces of `row` bytes, `stride` bytes apart (one piece: a plain vector).
+struct Span {
+  uintptr_t base;
+  int64_t rows, stride, row;
+};
+Span vec(const void* p, int64_t bytes) { return {reinterpret_cast<uintptr_t>(p), p != nullptr && bytes > 0, bytes, bytes}; }
+
+// Whether two buffers share a byte.  Rows of one stride may lie in each other's gaps (views of one
+// projection, vectors behind the rows of a table); with two strides any common range counts.
+bool overlap(Span a, Span b) {
+  if (a.rows <= 0 || b.rows <= 0 || a.row <= 0 || b.row <= 0) return false;
+  const uintptr_t a_end = a.base + (a.rows - 1) * a.stride + a.row, b_end = b.base + (b.rows - 1) * b.stride + b.row;
+  if (a.base >= b_end || b.base >= a_end) return false;
+  if (a.rows == 1) std::swap(a, b);
+  if (a.rows == 1 || (b.rows > 1 && a.stride != b.stride)) return true;
+  // b's start within a's rhythm of row and gap
+  const int64_t off = static_cast<int64_t>(b.base - a.base) % a.stride, at = off < 0 ? off + a.stride : off;
+  return at < a.row || at + b.row > a.stride;
+}
+
+// A plan's blocks read the lengths, the list and the table's old entries while others write the results.
+bool plan_overlaps(const hcp_step_plan_args& a) {
+  const int64_t reqs = 4 * static_cast<int64_t>(a.num_reqs), toks = a.num_tokens;
+  const Span in[] = {vec(a.context_lens, reqs), vec(a.new_lens, reqs), vec(a.pos_base, reqs),
+                     vec(a.free_blocks, 4 * a.num_free), vec(a.free_head, 4)};
+  const Span out[] = {vec(a.query_start, reqs + 4), vec(a.seq_lens, reqs), vec(a.positions, 8 * toks),
+                      vec(a.slot_mapping, 8 * toks), vec(a.token_req, 4 * toks), vec(a.kv_lens, 4 * toks),
+                      vec(a.free_head_out, 4), vec(a.missing_out, 4),
+                      Span{reinterpret_cast<uintptr_t>(a.block_table), a.num_reqs, 4 * a.block_table_stride,
+                           4 * a.block_table_width}};
+  for (const Span& o : out) {
+    for (const Span& i : in)
+      if (overlap(o, i)) return true;
+    for (const Span* p = out; p != &o; ++p)
+      if (overlap(o, *p)) return true;
+  }
+  return false;
+}
+
+}  // namespace
+
 extern "C" int hcp_kv_plan_step(const hcp_step_plan_args* a, void* stream) {
   if (!stream_on_current_device(stream)) return HCP_ERR_INVALID;
   if (a == nullptr || a->num_reqs < 0 || a->num_tokens < 0 || a->block_size <= 0 || a->block_table_width < 0 ||
@@ -912,6 +955,7 @@ extern "C" int hcp_kv_plan_step(const hcp_step_plan_args* a, void* stream) {
     return HCP_ERR_INVALID;
   if (a->num_tokens > INT32_MAX || a->block_table_width > INT32_MAX || a->num_free > INT32_MAX)
     return HCP_ERR_UNSUPPORTED;
+  if (plan_overlaps(*a)) return HCP_ERR_INVALID;
   StepPlanParams p;
   p.context_lens = a->context_lens;
   p.new_lens = a->new_lens;

@@ -286,6 +286,8 @@ int hcp_kv_cache_gather(const void* kv_cache, int64_t num_blocks, int32_t block_
  * Rows past the step's last token: position, slot and request -1, kv_len 0.
  * Only the new entries of block_table are written, so a call can be repeated.
  * *missing_out: blocks that were needed and not given (list or row exhausted).
+ * No output may share memory with an input or another output (HCP_ERR_INVALID):
+ * lengths are advanced by a copy of seq_lens after the call.
  *
  * Replaces: the host-side block and slot bookkeeping a serving engine does per
  * step before it calls do_kv_cache_update (hcp_vllm_plugin/ring_backend.py:
@@ -305,7 +307,7 @@ typedef struct hcp_step_plan_args {
   int64_t* slot_mapping;         /* [num_tokens] */
   int32_t* token_req;            /* [num_tokens] */
   int32_t* kv_lens;              /* [num_tokens] */
-  int32_t* free_head_out;        /* [1], may not alias free_head */
+  int32_t* free_head_out;        /* [1] */
   int32_t* missing_out;          /* [1] */
   int32_t num_reqs;
   int32_t block_size;

@@ -22,3 +22,35 @@ def test_chained_kernels_read_nothing_as_constant():
             for word in ("__ldg", "ld.global.nc", "__restrict__", "tex1Dfetch"):
                 assert word not in text, (name, word)
     assert chained == ["decode_q4.cuh", "norm_rope.cuh", "q4_cache.cuh", "step_plan.cuh"]
+
+
+def _addr(i):
+    return 0x7F0000000000 + i * 0x10000000
+
+
+def _args(cls, base, over):
+    a = cls()
+    for k, v in {**base, **over}.items():
+        setattr(a, k, v)
+    return a
+
+
+PLAN = dict(context_lens=_addr(1), new_lens=_addr(2), pos_base=_addr(14), block_table=_addr(3), block_table_stride=24,
+            block_table_width=8, free_blocks=_addr(4), num_free=9, free_head=_addr(5), query_start=_addr(6),
+            seq_lens=_addr(7), positions=_addr(8), slot_mapping=_addr(9), token_req=_addr(10), kv_lens=_addr(11),
+            free_head_out=_addr(12), missing_out=_addr(13), num_reqs=4, block_size=16, num_tokens=6)
+
+
+@pytest.mark.parametrize("over", [
+    dict(seq_lens=_addr(1)), dict(seq_lens=_addr(2)), dict(seq_lens=_addr(14) + 12), dict(query_start=_addr(1) - 16),
+    dict(query_start=_addr(2) + 12), dict(token_req=_addr(1)), dict(kv_lens=_addr(1) - 20), dict(positions=_addr(4)),
+    dict(slot_mapping=_addr(4) - 40), dict(missing_out=_addr(5)), dict(missing_out=_addr(4) + 32), dict(free_head_out=_addr(1)),
+    dict(missing_out=_addr(12)), dict(seq_lens=_addr(6) + 16), dict(kv_lens=_addr(10) + 20), dict(slot_mapping=_addr(8) + 40),
+    dict(seq_lens=_addr(3)), dict(context_lens=_addr(3) + 4 * (24 + 7)), dict(free_blocks=_addr(3) + 4 * (3 * 24 - 8)),
+    dict(positions=_addr(3) - 44), dict(free_head_out=_addr(3) + 4 * (3 * 24 + 7))])
+def test_plan_outputs_may_not_overlap(over):
+    """Blocks sum the lengths while others write the results: an output in the place of an input (or of
+    another output) is refused; advancing the lengths in place is the obvious one."""
+    a = _args(C.HcpStepPlanArgs, PLAN, over)
+    assert C.load().hcp_kv_plan_step(ctypes.byref(a), None) == 1
+

@@ -120,3 +120,21 @@ def test_decode_right_after_the_plan_sees_its_pages(ops):
         assert plan.missing.item() == 0
     for a, b in zip(outs, wants):
         assert torch.equal(a, b)
+
+
+def test_plan_takes_vectors_between_the_rows_of_a_table(ops):
+    """Rows of a wider buffer may hold the step's other vectors behind their table entries: nothing is shared."""
+    reqs, width, wide, bs = 5, 6, 20, 16
+    buf = torch.full((reqs, wide), -1, dtype=torch.int32, device="cuda")
+    context, new = np.array([0, 20, 33, 7, 64]), np.array([5, 1, 20, 0, 9])
+    buf[0, 8:13], buf[2, 10:15], buf[4, 7:8] = _i32(context), _i32(new), 2
+    table = np.full((reqs, width), -1, np.int32)
+    for i, c in enumerate(context):
+        table[i, : -(-c // bs)] = 100 + 10 * i + np.arange(-(-c // bs))
+    buf[:, :width] = _i32(table)
+    free = np.arange(40, 60)
+    want = R.plan(context, new, table, free, 2, bs, 40)
+    got = ops.kv_plan_step(buf[0, 8:13], buf[2, 10:15], buf[:, :width], _i32(free), buf[4, 7:8], block_size=bs, num_tokens=40)
+    for name, t in got._asdict().items():
+        np.testing.assert_array_equal(t.cpu().numpy(), want[name], err_msg=name)
+    np.testing.assert_array_equal(buf[:, :width].cpu().numpy(), want["block_table"])
