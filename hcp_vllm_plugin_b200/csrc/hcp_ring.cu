@@ -113,6 +113,13 @@ bool encode_rows_heads(CUtensorMap* m, bool f16, const void* base, int64_t rows,
   return encode_map(m, f16, 3, base, dims, strides, box);
 }
 
+// The status of a call that the runtime refused.  The error is this call's: a later call that asks for
+// the last error after its launch must not find it.
+int cuda_failed() {
+  cudaGetLastError();
+  return HCP_ERR_CUDA;
+}
+
 // Launch as a programmatic dependent of the kernel before it in the stream: for kernels of a
 // few microseconds that begin with ptx::chain_wait().  Their scheduling overlaps that kernel's end.
 template <typename... P>
@@ -127,7 +134,7 @@ int launch_chained(void (*kernel)(P...), dim3 grid, unsigned threads, int smem, 
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? HCP_OK : HCP_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? HCP_OK : cuda_failed();
 }
 
 std::mutex g_attr_mu;
@@ -1024,13 +1031,13 @@ template <int D, bool F16, int NT>
 int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
   constexpr int smem = sizeof(Dq4Smem<D>);
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return HCP_ERR_CUDA;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cuda_failed();
   {
     std::lock_guard<std::mutex> lk(g_attr_mu);
     bool& done = g_dq4_attr_done[D == 128][F16][NT == 2][dev];
     if (!done) {
       if (cudaFuncSetAttribute(decode_q4_kernel<D, F16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return HCP_ERR_CUDA;
+        return cuda_failed();
       done = true;
     }
   }

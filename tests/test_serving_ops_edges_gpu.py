@@ -138,3 +138,58 @@ def test_plan_takes_vectors_between_the_rows_of_a_table(ops):
     for name, t in got._asdict().items():
         np.testing.assert_array_equal(t.cpu().numpy(), want[name], err_msg=name)
     np.testing.assert_array_equal(buf[:, :width].cpu().numpy(), want["block_table"])
+
+
+# ------------------------------------------------------------------ calls that fail on the host
+
+class _Driver:
+    """The few driver calls that make a launch fail without reaching the GPU."""
+
+    def __init__(self):
+        import ctypes
+        self.lib, self.byref, self.ptr = ctypes.CDLL("libcuda.so.1"), ctypes.byref, ctypes.c_void_p
+        torch.zeros(1, device="cuda")  # torch's context is the current one
+
+    def __call__(self, name, *args):
+        rc = getattr(self.lib, name)(*args)
+        assert rc == 0, (name, rc)
+
+    def stream(self):
+        s = self.ptr()
+        self("cuStreamCreate", self.byref(s), 0)
+        return s
+
+
+def _plan_args(keep):
+    """Arguments of a small plan, and the tensors behind them."""
+    from hcp_vllm_plugin_b200 import _capi as C
+    i32 = lambda *x: keep.append(torch.tensor(x, dtype=torch.int32, device="cuda")) or keep[-1].data_ptr()  # noqa: E731
+    i64 = lambda n: keep.append(torch.zeros(n, dtype=torch.int64, device="cuda")) or keep[-1].data_ptr()  # noqa: E731
+    return C.HcpStepPlanArgs(context_lens=i32(3, 4), new_lens=i32(1, 1), block_table=i32(7, 8), block_table_stride=1,
+                             block_table_width=1, free_blocks=i32(9), num_free=1, free_head=i32(0), query_start=i32(0, 0, 0),
+                             seq_lens=i32(0, 0), positions=i64(2), slot_mapping=i64(2), token_req=i32(0, 0), kv_lens=i32(0, 0),
+                             free_head_out=i32(0), missing_out=i32(0), num_reqs=2, block_size=16, num_tokens=2)
+
+
+def test_a_failed_launch_is_reported_once(ops):
+    """A launch that the runtime refuses is that call's error, and no later call's."""
+    import ctypes
+
+    from hcp_vllm_plugin_b200 import _capi as C
+    lib, cu, keep = C.load(), _Driver(), []
+    a = _plan_args(keep)
+    k = torch.ones(2, 2, 64, dtype=BF16, device="cuda")
+    cache = torch.zeros(1, 2, 16, 128, dtype=BF16, device="cuda")
+    slots = torch.arange(2, device="cuda")
+    torch.cuda.synchronize()
+    # a stream that waits for the legacy one is being captured: nothing can be launched into the legacy stream
+    s, graph = cu.stream(), cu.ptr()
+    cu("cuStreamBeginCapture_v2", s, 0)
+    rc = lib.hcp_kv_plan_step(ctypes.byref(a), None)
+    cu.lib.cuStreamEndCapture(s, cu.byref(graph))
+    cu("cuStreamDestroy_v2", s)
+    assert rc not in (0, 1, 2), rc
+    ops.kv_cache_update(k, k, cache, slots)
+    torch.cuda.synchronize()
+    assert bool((cache[0, :, :2] == 1).all())
+    assert lib.hcp_kv_plan_step(ctypes.byref(a), None) == 0
