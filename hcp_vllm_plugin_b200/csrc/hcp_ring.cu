@@ -50,6 +50,36 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// A driver function as of CUDA 9.2, whose signatures these are (cuStreamGetCtx took a third argument later).
+template <typename F>
+F driver_entry(const char* name) {
+  void* ptr = nullptr;
+  cudaDriverEntryPointQueryResult q{};
+  return cudaGetDriverEntryPointByVersion(name, &ptr, 9020, cudaEnableDefault, &q) == cudaSuccess &&
+                 q == cudaDriverEntryPointSuccess
+             ? reinterpret_cast<F>(ptr)
+             : nullptr;
+}
+
+// Device of a captured stream, by its context.
+bool captured_stream_device(cudaStream_t st, int* dev) {
+  static const auto stream_ctx = driver_entry<CUresult (*)(CUstream, CUcontext*)>("cuStreamGetCtx");
+  static const auto current = driver_entry<CUresult (*)(CUcontext*)>("cuCtxGetCurrent");
+  static const auto push = driver_entry<CUresult (*)(CUcontext)>("cuCtxPushCurrent");
+  static const auto pop = driver_entry<CUresult (*)(CUcontext*)>("cuCtxPopCurrent");
+  static const auto device = driver_entry<CUresult (*)(CUdevice*)>("cuCtxGetDevice");
+  CUcontext ctx = nullptr, cur = nullptr;
+  if (stream_ctx == nullptr || current == nullptr || push == nullptr || pop == nullptr || device == nullptr) return false;
+  if (stream_ctx(st, &ctx) != CUDA_SUCCESS || current(&cur) != CUDA_SUCCESS) return false;
+  if (ctx == cur) return cudaGetDevice(dev) == cudaSuccess;
+  CUdevice d = -1;
+  if (push(ctx) != CUDA_SUCCESS) return false;
+  const bool ok = device(&d) == CUDA_SUCCESS;
+  pop(&cur);
+  *dev = d;
+  return ok;
+}
+
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Kernels launch on the current device.  A stream that belongs to another
@@ -57,16 +87,15 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 // addresses and tensor maps were made for that other device.  0, 1 and 2 are
 // the runtime's default / legacy / per-thread streams of the current device.
 // A stream that is being captured may not be asked for its device (the question
-// ends the capture); there the runtime itself refuses a launch from another device.
+// ends the capture); its context may, and the context knows the device.
 bool stream_on_current_device(void* stream) {
   if (reinterpret_cast<uintptr_t>(stream) <= 2) return true;
-  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture) == cudaSuccess &&
-      capture == cudaStreamCaptureStatusActive)
-    return true;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   int cur = -1, sdev = -1;
-  if (cudaGetDevice(&cur) != cudaSuccess) return false;
-  if (cudaStreamGetDevice(static_cast<cudaStream_t>(stream), &sdev) != cudaSuccess) {
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaGetDevice(&cur) != cudaSuccess || cudaStreamIsCapturing(st, &capture) != cudaSuccess ||
+      (capture == cudaStreamCaptureStatusActive ? !captured_stream_device(st, &sdev)
+                                                : cudaStreamGetDevice(st, &sdev) != cudaSuccess)) {
     cudaGetLastError();
     return false;
   }

@@ -193,3 +193,93 @@ def test_a_failed_launch_is_reported_once(ops):
     torch.cuda.synchronize()
     assert bool((cache[0, :, :2] == 1).all())
     assert lib.hcp_kv_plan_step(ctypes.byref(a), None) == 0
+
+
+def test_a_captured_stream_of_another_context_takes_nothing(ops):
+    """Kernels go to the current context alone: a captured stream of another one gets no launch, and the
+    calls after it are not affected."""
+    import ctypes
+
+    from hcp_vllm_plugin_b200 import _capi as C
+    lib, cu, keep = C.load(), _Driver(), []
+    a = _plan_args(keep)
+    torch.cuda.synchronize()
+    other, popped, graph = cu.ptr(), cu.ptr(), cu.ptr()
+    cu("cuCtxCreate_v2", cu.byref(other), 0, 0)   # current now
+    s = cu.stream()
+    cu("cuStreamBeginCapture_v2", s, 2)
+    cu("cuCtxPopCurrent_v2", cu.byref(popped))
+    rc = lib.hcp_kv_plan_step(ctypes.byref(a), s)
+    cu("cuCtxPushCurrent_v2", other)
+    cu.lib.cuStreamEndCapture(s, cu.byref(graph))
+    cu("cuStreamDestroy_v2", s)
+    cu("cuCtxPopCurrent_v2", cu.byref(popped))
+    cu("cuCtxDestroy_v2", other)
+    assert rc != 0
+    assert lib.hcp_kv_plan_step(ctypes.byref(a), None) == 0
+    torch.cuda.synchronize()
+
+
+def test_a_captured_stream_of_another_device_is_refused(ops):
+    """As outside of captures (HCP_ERR_INVALID), before anything is launched: the capture goes on."""
+    import ctypes
+
+    from hcp_vllm_plugin_b200 import _capi as C
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    lib, keep = C.load(), []
+    a = _plan_args(keep)
+    torch.cuda.synchronize()
+    x, graph = torch.zeros(4, device="cuda:1"), torch.cuda.CUDAGraph()
+    with torch.cuda.device(1):
+        with torch.cuda.graph(graph):
+            stream = torch.cuda.current_stream().cuda_stream
+            with torch.cuda.device(0):
+                rc = lib.hcp_kv_plan_step(ctypes.byref(a), stream)
+            x += 1
+        graph.replay()
+        torch.cuda.synchronize()
+    assert rc == 1 and x.tolist() == [1.0] * 4
+
+
+def test_every_entry_point_can_be_captured(ops):
+    """The attention, merge and 16-bit cache calls in one graph, replayed on new inputs: as eager, bit for bit."""
+    from hcp_vllm_plugin_b200 import _capi as C
+    gen = torch.Generator().manual_seed(31)
+    t, keys, h, hkv, d, bs = 300, 400, 28, 4, 128, 16
+    fresh = lambda *shape: torch.randn(*shape, generator=gen).to(BF16).cuda()  # noqa: E731
+    q, k, v, kc, vc = fresh(t, h, d), fresh(keys, hkv, d), fresh(keys, hkv, d), fresh(t, hkv, d), fresh(t, hkv, d)
+    cache, slots = torch.zeros(40, hkv, bs, 2 * d, dtype=BF16, device="cuda"), torch.randperm(640, generator=gen)[:t].cuda()
+    oa, ob, out = (torch.zeros(t, h, d, dtype=BF16, device="cuda") for _ in range(3))
+    la, lb, lse = (torch.zeros(h, t, device="cuda") for _ in range(3))
+    many, many_lse = torch.zeros(2, t, h, d, device="cuda"), torch.zeros(2, h, t, device="cuda")
+    joined = torch.zeros(t, h, d, dtype=BF16, device="cuda")
+
+    def run():
+        ops.kv_cache_update(kc, vc, cache, slots)
+        kg, vg = ops.kv_cache_gather(cache, slots)
+        ops.ring_attn_fwd(q, ops.make_work([(0, t, 0, 0, (C.HCP_SRC_A, 0, keys, -1), None)]), scale=0.1, num_kv_heads=hkv,
+                          out=oa, lse=la, k_a=k, v_a=v)
+        ops.ring_attn_fwd(q, ops.make_work([(0, t, 0, 0, (C.HCP_SRC_A, 0, t, 0), None)]), scale=0.1, num_kv_heads=hkv,
+                          out=ob, lse=lb, k_a=kg, v_a=vg)
+        ops.merge_attn_states(out, oa, la, ob, lb, output_lse=lse)
+        many[0].copy_(oa), many[1].copy_(ob), many_lse[0].copy_(la), many_lse[1].copy_(lb)
+        ops.merge_attn_states_n(joined, many, many_lse)
+        return [x.clone() for x in (cache, kg, vg, oa, ob, out, lse, joined)]
+
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for _ in range(2):
+        for x in (q, k, v, kc, vc):
+            x.copy_(torch.randn(x.shape, generator=gen))
+        slots.copy_(torch.randperm(640, generator=gen)[:t])
+        cache.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        held = [x.clone() for x in got]
+        cache.zero_()
+        for a, b in zip(held, run()):
+            assert torch.equal(a, b)
