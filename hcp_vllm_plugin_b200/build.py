@@ -6,7 +6,8 @@ The library links the CUDA runtime statically and resolves the driver's
 ``cuTensorMapEncodeTiled`` at run time, so it loads on any box with the
 NVIDIA driver and needs no torch at link time.  ``_hcp_front.so`` is the
 torch front end of the serving-step entry points (``csrc/front.cpp``, no
-kernels): an extension module for the installed torch and Python.
+kernels): an extension module for the installed torch and Python, left out
+where there is no torch.
 """
 
 from __future__ import annotations
@@ -46,7 +47,8 @@ def nvcc_path() -> str:
     return found
 
 
-def up_to_date(target: str = LIB, deps=DEPS) -> bool:
+def up_to_date(target: str | None = None, deps=DEPS) -> bool:
+    target = LIB if target is None else target
     if not os.path.exists(target):
         return False
     t = os.path.getmtime(target)
@@ -87,7 +89,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         _compile(cmd, LIB, verbose)
-    build_front(force, verbose)
+    try:
+        import torch  # noqa: F401
+    except ImportError as e:  # a host of the C ABI alone
+        print(f"{FRONT} is not built: it is the front end for torch, which cannot be imported ({e})", file=sys.stderr)
+    else:
+        build_front(force, verbose)
     return LIB
 
 
