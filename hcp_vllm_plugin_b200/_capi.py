@@ -260,10 +260,14 @@ def front():
         try:
             import torch  # noqa: F401 - brings the libraries that the module links
 
-            from . import _hcp_front as mod
+            from . import _hcp_front as mod, build
         except ImportError as e:
             raise HcpError(f"_hcp_front.so cannot be loaded ({e}): build it for this torch with "
                            "`python -m hcp_vllm_plugin_b200.build` (there is no fallback)") from e
+        built_for = getattr(mod, "built_for", "an unknown torch")
+        if built_for != build.front_target():
+            raise HcpError(f"_hcp_front.so was built for {built_for}, this is {build.front_target()}: build it anew "
+                           "with `python -m hcp_vllm_plugin_b200.build` (there is no fallback)")
         mod.bind(check, *(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
             "hcp_kv_plan_step", "hcp_qk_norm_rope", "hcp_kv_cache_update_q4", "hcp_kv_cache_gather_q4",
             "hcp_decode_q4_splitkv", "hcp_decode_q4_workspace_bytes")))

@@ -64,9 +64,24 @@ def _compile(cmd: list[str], target: str, verbose: bool) -> None:
     os.replace(tmp, target)
 
 
+def front_target() -> str:
+    """What the front end has to be built for; the module carries it (``built_for``)."""
+    import torch
+
+    return (f"torch {torch.__version__}, C++ ABI {int(torch._C._GLIBCXX_USE_CXX11_ABI)}, "
+            f"Python {sys.version_info.major}.{sys.version_info.minor} {sysconfig.get_config_var('SOABI')}")
+
+
+def _front_is_current() -> bool:
+    if not up_to_date(FRONT, [FRONT_SOURCE, HEADER]):
+        return False
+    with open(FRONT, "rb") as f:
+        return front_target().encode() in f.read()
+
+
 def build_front(force: bool = False, verbose: bool = False) -> str:
     """Compile the torch front end with the host compiler."""
-    if not force and up_to_date(FRONT, [FRONT_SOURCE, HEADER]):
+    if not force and _front_is_current():
         return FRONT
     import torch
 
@@ -75,7 +90,7 @@ def build_front(force: bool = False, verbose: bool = False) -> str:
     includes = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
                 os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include"), sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", os.path.join(ROOT, "include"),
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DHCP_BUILT_FOR="{front_target()}"', "-I", os.path.join(ROOT, "include"),
            *(a for p in includes for a in ("-isystem", p)), "-o", FRONT, FRONT_SOURCE,
            "-L", os.path.join(home, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
            "-ltorch_python"]

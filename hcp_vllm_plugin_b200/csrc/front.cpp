@@ -495,4 +495,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_hcp_front", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__hcp_front() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__hcp_front() {
+  PyObject* m = PyModule_Create(&module);
+  // the torch and Python that it was built for: another one's insides may differ
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", HCP_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

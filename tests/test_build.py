@@ -29,3 +29,30 @@ def test_the_library_is_built_without_torch(compiled, monkeypatch, capsys):
     assert B.build(force=True) == B.LIB
     assert compiled == [B.LIB]
     assert "_hcp_front.so" in capsys.readouterr().err
+
+
+def test_the_front_end_is_built_anew_for_another_torch(compiled, monkeypatch):
+    """Times of files do not tell which torch and Python a module was built for."""
+    import os
+
+    import torch
+    B.build_front()
+    assert compiled == [B.FRONT]
+    later = os.path.getmtime(B.FRONT_SOURCE) + 1e6
+    os.utime(B.FRONT, (later, later))
+    B.build_front()
+    assert compiled == [B.FRONT]               # up to date
+    monkeypatch.setattr(torch, "__version__", "0.0.1+other")
+    B.build_front()
+    assert compiled == [B.FRONT] * 2           # not for this torch
+    B.build_front()
+    assert compiled == [B.FRONT] * 2
+
+
+def test_a_front_end_built_for_another_torch_is_refused(monkeypatch):
+    from hcp_vllm_plugin_b200 import _capi
+    _capi.front()
+    monkeypatch.setattr(_capi, "_front", None)
+    monkeypatch.setattr(B, "front_target", lambda: "torch 0.0.1, another Python")
+    with pytest.raises(_capi.HcpError, match="built for torch"):
+        _capi.front()
