@@ -307,8 +307,9 @@ def _workspace(device: torch.device, nbytes: int) -> torch.Tensor:
     at the same time and must not share partials.  A captured call gets a
     buffer of its own: a graph keeps the address, which a cached one may
     lose when it grows, and graphs replayed at once must not share it."""
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    with torch.cuda.device(device):  # the capture of this GPU's stream is meant, not of the current GPU's
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
     key = (device.type, device.index, torch.cuda.current_stream(device).cuda_stream)
     buf = _workspaces.get(key)
     if buf is None or buf.numel() < nbytes:
