@@ -1153,6 +1153,17 @@ extern "C" int hcp_qk_norm_rope(const hcp_norm_rope_args* a, void* stream) {
     return HCP_ERR_INVALID;
   if ((a->q_weight != nullptr && !aligned8(a->q_weight)) || (a->k_weight != nullptr && !aligned8(a->k_weight)))
     return HCP_ERR_INVALID;
+  // a result may replace its own input, and nothing else that is read
+  auto rows = [&](const void* base, int64_t stride, int64_t row) {
+    return Span{reinterpret_cast<uintptr_t>(base), a->num_tokens, 2 * stride, 2 * row};
+  };
+  const Span q = rows(a->q, a->q_row_stride, q_row), k = rows(a->k, a->k_row_stride, kv_row),
+             v = cached ? rows(a->v, a->v_row_stride, kv_row) : Span{}, qo = rows(a->q_out, a->q_out_row_stride, q_row),
+             ko = rows(a->k_out, a->k_out_row_stride, kv_row);
+  auto own = [](const Span& out, const Span& in) { return out.base == in.base && (out.rows <= 1 || out.stride == in.stride); };
+  if ((!own(qo, q) && overlap(qo, q)) || (!own(ko, k) && overlap(ko, k)) || overlap(qo, k) || overlap(ko, q) ||
+      overlap(qo, v) || overlap(ko, v) || overlap(qo, ko))
+    return HCP_ERR_INVALID;
   NormRopeParams p;
   p.q = static_cast<const uint16_t*>(a->q);
   p.k = static_cast<const uint16_t*>(a->k);

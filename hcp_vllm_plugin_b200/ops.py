@@ -524,7 +524,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, cos_
     [num_blocks, Hkv, block_size, 2*D] or the 4-bit one
     (:func:`kv_cache_q4_shape`), slot_mapping [T] int64 as in
     :func:`kv_cache_update`.  Returns (q_out, k_out), allocated unless given;
-    they may be q and k themselves.
+    they may be q and k themselves, and may share no other memory with q, k, value
+    or each other.
 
     Rows with a negative position are padding and stay as they were; positions
     past the table give NaN rows and write no slot.

@@ -323,7 +323,8 @@ int hcp_kv_plan_step(const hcp_step_plan_args* args, void* stream);
  *   dims (i, i + rotary / 2), or (2i, 2i + 1) with interleaved != 0; dims past
  *   `rotary` keep y.  cos_sin [table_rows, rotary]: cos, then sin.
  * 32-bit arithmetic, one rounding to dtype; the cache holds the rounded keys.
- * q_out / k_out may be q / k themselves.  A negative position marks a padding
+ * q_out / k_out may be q / k themselves; sharing any other memory with q, k, v or
+ * each other is refused (HCP_ERR_INVALID).  A negative position marks a padding
  * row: its outputs and slot stay as they were.  A position past the table gives
  * NaN rows and leaves its slot.  Slots as in hcp_kv_cache_update.
  */

@@ -54,3 +54,26 @@ def test_plan_outputs_may_not_overlap(over):
     a = _args(C.HcpStepPlanArgs, PLAN, over)
     assert C.load().hcp_kv_plan_step(ctypes.byref(a), None) == 1
 
+
+
+# q, k and v of one projection: 8 query heads, 2 KV heads of 128 dims, rows of 12 heads
+QKV = _addr(1)
+ROPE = dict(dtype=C.HCP_BF16, num_heads=8, num_kv_heads=2, head_dim=128, q=QKV, q_row_stride=1536, k=QKV + 2048,
+            k_row_stride=1536, v=QKV + 2560, v_row_stride=1536, q_out=_addr(4), q_out_row_stride=1024, k_out=_addr(5),
+            k_out_row_stride=256, positions=_addr(6), num_tokens=4, cos_sin=_addr(7), table_rows=100, table_stride=128,
+            table_dtype=C.HCP_F32, rotary=128, interleaved=0, eps=1e-6, q_weight=_addr(8), k_weight=_addr(9),
+            kv_cache=_addr(10), slot_mapping=_addr(11), num_blocks=9, block_size=16, cache_kind=C.HCP_ROPE_CACHE_SAME)
+
+
+@pytest.mark.parametrize("over", [
+    dict(v=QKV + 2048, k_out=QKV + 2048, k_out_row_stride=1536),        # values in the place of the keys' results
+    dict(k_out=QKV + 2560, k_out_row_stride=1536),                      # the keys' results in the place of the values
+    dict(k_out=QKV + 2560, k_out_row_stride=1536, cache_kind=C.HCP_ROPE_CACHE_Q4),
+    dict(k_out=QKV + 2304, k_out_row_stride=1536), dict(k_out=QKV, k_out_row_stride=1536),
+    dict(q_out=QKV + 256, q_out_row_stride=1536), dict(q_out=QKV, q_out_row_stride=1024),
+    dict(q_out=QKV + 1024, q_out_row_stride=1536), dict(k_out=QKV + 2048, k_out_row_stride=256),
+    dict(k_out=_addr(4) + 512, k_out_row_stride=1024), dict(q_out=_addr(5) - 2048, q_out_row_stride=1024)])
+def test_norm_rope_outputs_may_not_overlap_other_rows(over):
+    """Results may stand in the place of their own inputs; anywhere else in q, k or v, or in each other,
+    what is read depends on what was written before."""
+    assert C.load().hcp_qk_norm_rope(ctypes.byref(_args(C.HcpNormRopeArgs, ROPE, over)), None) == 1

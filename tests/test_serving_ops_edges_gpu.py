@@ -283,3 +283,38 @@ def test_every_entry_point_can_be_captured(ops):
         cache.zero_()
         for a, b in zip(held, run()):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ results in the place of inputs
+
+@pytest.mark.parametrize("kind", ["same", "q4"])
+@pytest.mark.parametrize("t", [1, 45, 700])
+def test_norm_rope_in_place_beside_the_values(ops, kind, t):
+    """q and k of one projection's output turned where they stand, with the values behind them going into the
+    cache: as with results of their own.  One tensor as keys and values will do where the results stand elsewhere."""
+    gen = torch.Generator().manual_seed(t)
+    h, hkv, d, bs = 8, 2, 128, 16
+    qkv = torch.randn(t, (h + 2 * hkv) * d, generator=gen).to(BF16).cuda()
+    nb = t // bs + 2
+    shape = (nb, hkv, bs, 2 * d) if kind == "same" else ops.kv_cache_q4_shape(nb, hkv, bs, d)
+    dtype = BF16 if kind == "same" else torch.uint8
+    pos, slots = torch.randint(0, 90, (t,), generator=gen).cuda(), torch.randperm(nb * bs, generator=gen)[:t].cuda()
+    angle = torch.rand(90, d // 2, generator=gen, dtype=torch.float64) * 6
+    table = torch.cat([angle.cos(), angle.sin()], -1).float().cuda()
+    w = (1 + 0.2 * torch.randn(d, generator=gen)).to(BF16).cuda()
+
+    def run(buf, in_place, shared=False):
+        q, k, v = (x.view(t, -1, d) for x in buf.split([h * d, hkv * d, hkv * d], -1))
+        cache = torch.zeros(shape, dtype=dtype, device="cuda")
+        out = dict(q_out=q, k_out=k) if in_place else {}
+        a, b = ops.qk_norm_rope(q, k, pos, table, q_weight=w, k_weight=w, value=k if shared else v, kv_cache=cache,
+                                slot_mapping=slots, **out)
+        return a.clone(), b.clone(), v.clone(), cache
+
+    for x, y in zip(run(qkv.clone(), False), run(qkv.clone(), True)):
+        assert torch.equal(x, y)
+    _, k_out, _, cache = run(qkv.clone(), False, shared=True)
+    want = torch.zeros_like(cache)
+    raw = qkv[:, h * d: (h + hkv) * d].view(t, hkv, d)
+    (ops.kv_cache_update if kind == "same" else ops.kv_cache_update_q4)(k_out, raw, want, slots)
+    assert torch.equal(cache.view(torch.uint8), want.view(torch.uint8))
