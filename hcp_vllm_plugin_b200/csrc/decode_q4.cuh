@@ -392,7 +392,8 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
         sq[nt][a][0] = 16.f * __shfl_sync(0xffffffffu, part[a], 8 * t);
         sq[nt][a][1] = 16.f * __shfl_sync(0xffffffffu, part[a], 8 * t + 4);
       }
-      const float down = 0.0625f * p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+      // at least the smallest number of 32 bits: with 0 an absent key's -inf would be NaN (scores of 2^-22 at most stay)
+      const float down = fmaxf(0.0625f * p.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 - e) << 23), 0x1p-149f);
       hs[nt][0] = __shfl_sync(0xffffffffu, down, 8 * t);
       hs[nt][1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
     }

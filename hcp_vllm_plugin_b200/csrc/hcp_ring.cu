@@ -1085,6 +1085,8 @@ int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
   return launch_chained(decode_q4_join_wide_kernel<D, D / 32, 8>, grid, threads, 0, st, p);
 }
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 int validate_decode_q4(const hcp_decode_q4_args* a) {
   if (a == nullptr) return HCP_ERR_INVALID;
   if (a->dtype != HCP_BF16 && a->dtype != HCP_F16) return HCP_ERR_UNSUPPORTED;
@@ -1092,7 +1094,7 @@ int validate_decode_q4(const hcp_decode_q4_args* a) {
   if (H <= 0 || Hkv <= 0 || H % Hkv != 0) return HCP_ERR_INVALID;
   if (H / Hkv > kDecMaxGroup || (D != 64 && D != 128) || !q4_block_size(a->block_size)) return HCP_ERR_UNSUPPORTED;
   if (a->out_dtype != a->dtype && a->out_dtype != HCP_F32) return HCP_ERR_UNSUPPORTED;
-  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return HCP_ERR_INVALID;
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale * kLog2e)) return HCP_ERR_INVALID;
   if (a->q_rows < 0) return HCP_ERR_INVALID;
   if (a->q_rows > INT32_MAX / 2 / Hkv) return HCP_ERR_UNSUPPORTED;
   if (a->q_rows == 0) return HCP_OK;
@@ -1324,7 +1326,7 @@ extern "C" int hcp_decode_q4_splitkv(const hcp_decode_q4_args* a, void* stream) 
   p.group = G;
   p.block_size = a->block_size;
   p.sub_shift = pow2_shift(a->block_size / kQ4TileTokens);
-  p.scale_log2 = a->scale * 1.4426950408889634f;
+  p.scale_log2 = a->scale * kLog2e;
   p.out_dt = a->out_dtype;
   p.out_vec = aligned16(a->out) && a->out_row_stride % (a->out_dtype == HCP_F32 ? 4 : 8) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -398,7 +398,7 @@ typedef struct hcp_decode_q4_args {
   int32_t num_heads;
   int32_t num_kv_heads;          /* num_heads / num_kv_heads <= 16 */
   int32_t head_dim;              /* 64 or 128 */
-  float scale;
+  float scale;                   /* > 0, and finite times log2(e) */
   int32_t block_size;            /* 16, 32, 64 or 128 */
   const void* q;                 int64_t q_rows; int64_t q_row_stride;
   const void* kv_cache;          int64_t num_blocks;

@@ -77,3 +77,19 @@ def test_norm_rope_outputs_may_not_overlap_other_rows(over):
     """Results may stand in the place of their own inputs; anywhere else in q, k or v, or in each other,
     what is read depends on what was written before."""
     assert C.load().hcp_qk_norm_rope(ctypes.byref(_args(C.HcpNormRopeArgs, ROPE, over)), None) == 1
+
+
+DECODE = dict(dtype=C.HCP_BF16, num_heads=28, num_kv_heads=4, head_dim=128, scale=0.1, block_size=16, q=_addr(1), q_rows=3,
+              q_row_stride=28 * 128, kv_cache=_addr(2), num_blocks=9, block_table=_addr(3), block_table_rows=3,
+              block_table_stride=8, block_table_width=8, kv_lens=_addr(4), token_req=None, out=_addr(5),
+              out_row_stride=28 * 128, out_dtype=C.HCP_BF16, lse=_addr(6), lse_stride=3, workspace=_addr(7),
+              workspace_bytes=1 << 40)
+
+
+@pytest.mark.parametrize("scale,taken", [(1e-44, True), (2e38, True), (2.4e38, False), (3.4e38, False)])
+def test_decode_q4_scale_range(scale, taken):
+    """Scores are kept in powers of two: a scale times log2(e) has to be finite in 32 bits."""
+    a = _args(C.HcpDecodeQ4Args, DECODE, dict(scale=scale))
+    assert (C.load().hcp_decode_q4_workspace_bytes(ctypes.byref(a)) > 0) == taken
+    if not taken:
+        assert C.load().hcp_decode_q4_splitkv(ctypes.byref(a), None) == 1

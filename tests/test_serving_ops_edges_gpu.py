@@ -318,3 +318,28 @@ def test_norm_rope_in_place_beside_the_values(ops, kind, t):
     raw = qkv[:, h * d: (h + hkv) * d].view(t, hkv, d)
     (ops.kv_cache_update if kind == "same" else ops.kv_cache_update_q4)(k_out, raw, want, slots)
     assert torch.equal(cache.view(torch.uint8), want.view(torch.uint8))
+
+
+# ------------------------------------------------------------------ the smallest scales
+
+@pytest.mark.parametrize("h,hkv,d,dtype", [(28, 4, 128, BF16), (12, 1, 64, F16)])
+@pytest.mark.parametrize("scale,size", [(1e-44, 1.0), (1e-30, 1.0), (1e-12, 1e-38)])
+def test_decode_q4_scales_that_vanish(ops, scale, size, h, hkv, d, dtype):
+    """A scale (or a query) so small that their product leaves 32 bits: every key weighs the same, and keys that
+    are not there still weigh nothing."""
+    if dtype == F16 and size != 1.0:
+        size = 2.0 ** -24
+    gen = torch.Generator().manual_seed(33)
+    bs, nb, lens = 16, 30, [1, 7, 16, 33, 470]
+    n = nb * bs
+    cache = torch.full(ops.kv_cache_q4_shape(nb, hkv, bs, d), 0xFF, dtype=torch.uint8, device="cuda")
+    k, v = (torch.randn(480, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    ops.kv_cache_update_q4(k[:470].cuda(), v[:470].cuda(), cache, torch.arange(470, device="cuda"))
+    kq, vq = R.read_q4(cache.cpu().numpy(), np.arange(470), dtype)
+    q = (torch.randn(len(lens), h, d, generator=gen).double() * size).to(dtype)
+    table = torch.arange(nb, dtype=torch.int32, device="cuda").view(1, nb)
+    out, lse = torch.zeros(len(lens), h, d, device="cuda"), torch.zeros(h, len(lens), device="cuda")
+    ops.decode_splitkv_q4(q.cuda(), cache, table, _i32(lens), scale=scale, out=out, lse=lse, token_req=_i32([0] * len(lens)))
+    o, l = R.f64(out), R.f64(lse)
+    for r, n in enumerate(lens):
+        _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq[:n], vq[:n], scale, torch.float32, (scale, n))
