@@ -62,6 +62,10 @@ constexpr int kDq4MaxPieces = kDq4MaxCtas * kDq4Warps;
 constexpr int kDq4Stages = 3;    // steps of a warp's ring: one read, the others in flight
 constexpr int kDq4Step = 2;      // tiles of a step, and of a piece at least
 constexpr int kDq4JoinWarps = 16;
+constexpr int kDq4JoinThreads = 256;                          // of a join block where pairs are many
+constexpr int kDq4FewParts = 32;                              // of a pair that a warp joins alone
+constexpr int kDq4MaxLong = 2 * kDq4MaxPieces / kDq4FewParts; // pairs of more: a piece has parts of two pairs at most
+constexpr int kDq4Lookers = 32;                               // blocks a head that look for them
 constexpr int kDq4UnitTop = 127 + 118;  // exponent of the finest unit's reciprocal: p_j <= 2^8 times it stays finite
 // Blocks of an SM: 168 registers a thread, and twice the sums beyond 8 heads a group.
 constexpr int dq4_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
@@ -720,11 +724,10 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
   }
 }
 
-// Joins the parts of (row, KV head) blockIdx.x; sums run in a fixed order.
-__device__ __forceinline__ bool dq4_parts(const DecodeQ4Params& p, int4& desc) {
-  ptx::chain_wait();
-  ptx::chain_next();
-  desc = p.desc[blockIdx.x];
+// ---- joins of a (row, KV head)'s parts; sums run in a fixed order
+// That pair's parts, and whether there are any.
+__device__ __forceinline__ bool dq4_parts(const DecodeQ4Params& p, int pair, int4& desc) {
+  desc = p.desc[pair];
   return desc.z > 0 && desc.x >= 0 && desc.x + desc.z <= kDq4MaxPieces && (desc.y & ~1) == 0;
 }
 __device__ __forceinline__ long long dq4_part(const int4& desc, int i, int G, int h) {
@@ -734,126 +737,155 @@ __device__ __forceinline__ float dq4_lse(float M, float ls) {
   return ls == 0.f ? -INFINITY : (M + lg2_approx(ls)) * 0.69314718055994530942f;
 }
 
-// Many pairs, each of few parts: a warp takes a head of the pair and all its parts.
+// A warp takes a head of the pair and all its parts.
 template <int D>
-__global__ void __launch_bounds__(256) decode_q4_join_kernel(const __grid_constant__ DecodeQ4Params p) {
-  int4 desc;
-  if (!dq4_parts(p, desc)) return;
+__device__ __forceinline__ void dq4_join_few(const DecodeQ4Params& p, const int4 desc, int pair, int h) {
   constexpr int V = D / 32;  // neighbouring dims of a lane
   const int G = p.group, lane = threadIdx.x & 31;
-  const int row = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
-  for (int h = threadIdx.x >> 5; h < G; h += blockDim.x >> 5) {
-    float M = -INFINITY;
-    for (int i = lane; i < desc.z; i += 32) M = fmaxf(M, p.part_ml[dq4_part(desc, i, G, h)].x);
-#pragma unroll
-    for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-    float acc[V], ls = 0.f;
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.f;
-    if (M != -INFINITY) {
-#pragma unroll 8
-      for (int i = 0; i < desc.z; ++i) {
-        const long long at = dq4_part(desc, i, G, h);
-        const float2 ml = p.part_ml[at];
-        const float x = ex2_approx(ml.x - M);
-        ls = fmaf(x, ml.y, ls);
-        const float* part = p.part_o + at * D + V * lane;
-        if constexpr (V == 4) {
-          const float4 o = *reinterpret_cast<const float4*>(part);
-          acc[0] = fmaf(x, o.x, acc[0]);
-          acc[1] = fmaf(x, o.y, acc[1]);
-          acc[2] = fmaf(x, o.z, acc[2]);
-          acc[3] = fmaf(x, o.w, acc[3]);
-        } else {
-          const float2 o = *reinterpret_cast<const float2*>(part);
-          acc[0] = fmaf(x, o.x, acc[0]);
-          acc[1] = fmaf(x, o.y, acc[1]);
-        }
-      }
-    }
-    const int head = kvh * G + h;
-#pragma unroll
-    for (int v = 0; v < V; ++v) dq4_store(p, row, head, D, V * lane + v, ls == 0.f ? 0.f : acc[v] / ls);
-    if (lane == 0 && p.lse != nullptr) p.lse[head * p.lse_stride + row] = dq4_lse(M, ls);
-  }
-}
-
-// Few pairs, each of many parts: a block takes 32 V dims (blockIdx.z) of one head (blockIdx.y) and
-// its warps share the parts, P each at a time, all loaded before the first weight is known.  The
-// parts were just written by other SMs, so the reads' latency is what this costs.
-template <int D, int V, int P>
-__global__ void __launch_bounds__(kDq4JoinWarps * 32) decode_q4_join_wide_kernel(const __grid_constant__ DecodeQ4Params p) {
-  int4 desc;
-  if (!dq4_parts(p, desc)) return;
-  __shared__ float weight[kDq4MaxPieces], red[kDq4JoinWarps], sum[kDq4JoinWarps], so[kDq4JoinWarps][32 * V];
-  const int G = p.group, h = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
-  const float* const part = p.part_o + (blockIdx.z * 32 + lane) * V;
-  float o[P][V];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      const int i = i0 + j * warps;
-#pragma unroll
-      for (int v = 0; v < V; ++v) o[j][v] = 0.f;
-      if (i >= desc.z) continue;
-      const float* at = part + dq4_part(desc, i, G, h) * D;
-      if constexpr (V == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(at);
-        o[j][0] = x.x; o[j][1] = x.y; o[j][2] = x.z; o[j][3] = x.w;
-      } else if constexpr (V == 2) {
-        const float2 x = *reinterpret_cast<const float2*>(at);
-        o[j][0] = x.x; o[j][1] = x.y;
-      } else {
-        o[j][0] = *at;
-      }
-    }
-  };
-  load(warp);
+  const int row = pair / p.num_kv_heads, kvh = pair % p.num_kv_heads;
   float M = -INFINITY;
-  for (int i = tid; i < desc.z; i += blockDim.x) M = fmaxf(M, p.part_ml[dq4_part(desc, i, G, h)].x);
+  for (int i = lane; i < desc.z; i += 32) M = fmaxf(M, p.part_ml[dq4_part(desc, i, G, h)].x);
 #pragma unroll
   for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
-  if (lane == 0) red[warp] = M;
-  __syncthreads();
-  M = red[0];
-  for (int w = 1; w < warps; ++w) M = fmaxf(M, red[w]);
-  const float base = M == -INFINITY ? 0.f : M;
-  float ls = 0.f;
-  for (int i = tid; i < desc.z; i += blockDim.x) {
-    const float2 ml = p.part_ml[dq4_part(desc, i, G, h)];
-    const float x = ex2_approx(ml.x - base);
-    weight[i] = x;
-    ls = fmaf(x, ml.y, ls);
-  }
-#pragma unroll
-  for (int s = 16; s > 0; s >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, s);
-  if (lane == 0) sum[warp] = ls;
-  __syncthreads();
-  float acc[V];
+  float acc[V], ls = 0.f;
 #pragma unroll
   for (int v = 0; v < V; ++v) acc[v] = 0.f;
-  for (int i0 = warp; i0 < desc.z; i0 += P * warps) {
-    if (i0 != warp) load(i0);
-#pragma unroll
-    for (int j = 0; j < P; ++j) {
-      if (i0 + j * warps >= desc.z) break;
-      const float x = weight[i0 + j * warps];
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = fmaf(x, o[j][v], acc[v]);
+  if (M != -INFINITY) {
+#pragma unroll 8
+    for (int i = 0; i < desc.z; ++i) {
+      const long long at = dq4_part(desc, i, G, h);
+      const float2 ml = p.part_ml[at];
+      const float x = ex2_approx(ml.x - M);
+      ls = fmaf(x, ml.y, ls);
+      const float* part = p.part_o + at * D + V * lane;
+      if constexpr (V == 4) {
+        const float4 o = *reinterpret_cast<const float4*>(part);
+        acc[0] = fmaf(x, o.x, acc[0]);
+        acc[1] = fmaf(x, o.y, acc[1]);
+        acc[2] = fmaf(x, o.z, acc[2]);
+        acc[3] = fmaf(x, o.w, acc[3]);
+      } else {
+        const float2 o = *reinterpret_cast<const float2*>(part);
+        acc[0] = fmaf(x, o.x, acc[0]);
+        acc[1] = fmaf(x, o.y, acc[1]);
+      }
     }
   }
+  const int head = kvh * G + h;
 #pragma unroll
-  for (int v = 0; v < V; ++v) so[warp][lane * V + v] = acc[v];
-  __syncthreads();
-  const int row = blockIdx.x / p.num_kv_heads, head = blockIdx.x % p.num_kv_heads * G + h;
-  ls = 0.f;
-  for (int w = 0; w < warps; ++w) ls += sum[w];
-  for (int d = tid; d < 32 * V; d += blockDim.x) {
-    float v = 0.f;
-    for (int w = 0; w < warps; ++w) v += so[w][d];
-    dq4_store(p, row, head, D, blockIdx.z * 32 * V + d, ls == 0.f ? 0.f : v / ls);
+  for (int v = 0; v < V; ++v) dq4_store(p, row, head, D, V * lane + v, ls == 0.f ? 0.f : acc[v] / ls);
+  if (lane == 0 && p.lse != nullptr) p.lse[head * p.lse_stride + row] = dq4_lse(M, ls);
+}
+
+// A block takes 32 V dims (blockIdx.z) of one head of a pair and its warps share the parts, P each at a
+// time, all loaded before the first weight is known.  The parts were just written by other SMs, so the
+// reads' latency is what this costs.
+//   Few pairs, each of many parts (LOOK false): a block a pair (blockIdx.x) and head (blockIdx.y).
+//   Many pairs, most of few parts (LOOK): the first blocks look through a share of the pairs, one head each,
+// for those of more parts than a warp should take alone (one long row among many short ones: 440 parts to a
+// pair at 128k keys); the warps of the blocks after them take a head of a pair each.  Measured (28/4 heads,
+// D 128, the whole call): one row of 131072 keys among 31 of 300 takes 95 us with a warp for every head and
+// pair, 38 us so.
+template <int D, int V, int P, bool LOOK>
+__global__ void __launch_bounds__(LOOK ? kDq4JoinThreads : kDq4JoinWarps * 32, LOOK ? 4 : 1)
+    decode_q4_join_kernel(const __grid_constant__ DecodeQ4Params p) {
+  __shared__ float weight[kDq4MaxPieces], red[kDq4JoinWarps], sum[kDq4JoinWarps], so[kDq4JoinWarps][32 * V];
+  __shared__ int found, list[LOOK ? kDq4MaxLong : 1];
+  ptx::chain_wait();
+  ptx::chain_next();
+  const int G = p.group, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, warps = blockDim.x >> 5;
+  const int h = LOOK ? blockIdx.x % G : blockIdx.y;
+  int4 desc;
+  if constexpr (LOOK) {
+    const int pairs = p.rows * p.num_kv_heads, lookers = kDq4Lookers * G;
+    if (blockIdx.x >= lookers) {
+      const long long at = static_cast<long long>(blockIdx.x - lookers) * warps + warp;
+      const int pair = static_cast<int>(at / G);
+      if (pair < pairs && dq4_parts(p, pair, desc) && desc.z <= kDq4FewParts) dq4_join_few<D>(p, desc, pair, static_cast<int>(at % G));
+      return;
+    }
+    if (tid == 0) found = 0;
+    __syncthreads();
+    for (int i = blockIdx.x / G + kDq4Lookers * tid; i < pairs; i += kDq4Lookers * blockDim.x)
+      if (p.desc[i].z > kDq4FewParts) {
+        const int at = atomicAdd(&found, 1);  // in any order: each is joined by itself
+        if (at < kDq4MaxLong) list[at] = i;
+      }
+    __syncthreads();
   }
-  if (tid == 0 && blockIdx.z == 0 && p.lse != nullptr) p.lse[head * p.lse_stride + row] = dq4_lse(M, ls);
+  const int count = LOOK ? min(found, kDq4MaxLong) : 1;
+  for (int k = 0; k < count; ++k) {
+    const int pair = LOOK ? list[k] : static_cast<int>(blockIdx.x);
+    if (!dq4_parts(p, pair, desc)) continue;
+    const float* const part = p.part_o + (blockIdx.z * 32 + lane) * V;
+    float o[P][V];
+    auto load = [&](int i0) {
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        const int i = i0 + j * warps;
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[j][v] = 0.f;
+        if (i >= desc.z) continue;
+        const float* at = part + dq4_part(desc, i, G, h) * D;
+        if constexpr (V == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(at);
+          o[j][0] = x.x; o[j][1] = x.y; o[j][2] = x.z; o[j][3] = x.w;
+        } else if constexpr (V == 2) {
+          const float2 x = *reinterpret_cast<const float2*>(at);
+          o[j][0] = x.x; o[j][1] = x.y;
+        } else {
+          o[j][0] = *at;
+        }
+      }
+    };
+    load(warp);
+    float M = -INFINITY;
+    for (int i = tid; i < desc.z; i += blockDim.x) M = fmaxf(M, p.part_ml[dq4_part(desc, i, G, h)].x);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, s));
+    if (lane == 0) red[warp] = M;
+    __syncthreads();
+    M = red[0];
+    for (int w = 1; w < warps; ++w) M = fmaxf(M, red[w]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float ls = 0.f;
+    for (int i = tid; i < desc.z; i += blockDim.x) {
+      const float2 ml = p.part_ml[dq4_part(desc, i, G, h)];
+      const float x = ex2_approx(ml.x - base);
+      weight[i] = x;
+      ls = fmaf(x, ml.y, ls);
+    }
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) ls += __shfl_xor_sync(0xffffffffu, ls, s);
+    if (lane == 0) sum[warp] = ls;
+    __syncthreads();
+    float acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = 0.f;
+    for (int i0 = warp; i0 < desc.z; i0 += P * warps) {
+      if (i0 != warp) load(i0);
+#pragma unroll
+      for (int j = 0; j < P; ++j) {
+        if (i0 + j * warps >= desc.z) break;
+        const float x = weight[i0 + j * warps];
+#pragma unroll
+        for (int v = 0; v < V; ++v) acc[v] = fmaf(x, o[j][v], acc[v]);
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < V; ++v) so[warp][lane * V + v] = acc[v];
+    __syncthreads();
+    const int row = pair / p.num_kv_heads, head = pair % p.num_kv_heads * G + h;
+    ls = 0.f;
+    for (int w = 0; w < warps; ++w) ls += sum[w];
+    for (int d = tid; d < 32 * V; d += blockDim.x) {
+      float v = 0.f;
+      for (int w = 0; w < warps; ++w) v += so[w][d];
+      dq4_store(p, row, head, D, blockIdx.z * 32 * V + d, ls == 0.f ? 0.f : v / ls);
+    }
+    if (tid == 0 && blockIdx.z == 0 && p.lse != nullptr) p.lse[head * p.lse_stride + row] = dq4_lse(M, ls);
+    if constexpr (LOOK) __syncthreads();
+  }
 }
 
 }  // namespace hcp

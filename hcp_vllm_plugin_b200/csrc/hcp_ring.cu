@@ -1076,13 +1076,15 @@ int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
   const int64_t parts = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps / pairs + 2;  // of a pair, were the rows alike
   // From about 16 parts on they are shared between warps, 8 each; where the heads alone leave SMs
   // idle, a head's dims are split over blocks too (parts are many then).
-  const bool wide = parts >= 16, split = pairs * p.group < kDq4Sms;
-  const dim3 grid(static_cast<unsigned>(pairs), wide ? static_cast<unsigned>(p.group) : 1u, split ? D / 32 : 1);
-  const unsigned threads = 32 * (wide ? static_cast<unsigned>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8))
-                                      : static_cast<unsigned>(std::min(p.group, 8)));
-  if (!wide) return launch_chained(decode_q4_join_kernel<D>, grid, threads, 0, st, p);
-  if (split) return launch_chained(decode_q4_join_wide_kernel<D, 1, 32>, grid, threads, 0, st, p);
-  return launch_chained(decode_q4_join_wide_kernel<D, D / 32, 8>, grid, threads, 0, st, p);
+  if (parts < 16) {
+    const int64_t blocks = kDq4Lookers * p.group + (pairs * p.group + kDq4JoinThreads / 32 - 1) / (kDq4JoinThreads / 32);
+    return launch_chained(decode_q4_join_kernel<D, D / 32, 8, true>, dim3(static_cast<unsigned>(blocks)), kDq4JoinThreads, 0, st, p);
+  }
+  const bool split = pairs * p.group < kDq4Sms;
+  const dim3 grid(static_cast<unsigned>(pairs), static_cast<unsigned>(p.group), split ? D / 32 : 1);
+  const unsigned threads = 32 * static_cast<unsigned>(std::min<int64_t>(kDq4JoinWarps, (parts + 7) / 8));
+  if (split) return launch_chained(decode_q4_join_kernel<D, 1, 32, false>, grid, threads, 0, st, p);
+  return launch_chained(decode_q4_join_kernel<D, D / 32, 8, false>, grid, threads, 0, st, p);
 }
 
 constexpr float kLog2e = 1.4426950408889634f;

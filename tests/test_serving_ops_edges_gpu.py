@@ -343,3 +343,29 @@ def test_decode_q4_scales_that_vanish(ops, scale, size, h, hkv, d, dtype):
     o, l = R.f64(out), R.f64(lse)
     for r, n in enumerate(lens):
         _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq[:n], vq[:n], scale, torch.float32, (scale, n))
+
+
+# ------------------------------------------------------------------ joins
+
+@pytest.mark.parametrize("h,hkv,d,dtype,rows,longest", [
+    (28, 4, 128, BF16, 24, 60000), (4, 4, 64, BF16, 32, 900), (4, 4, 128, F16, 36, 700), (32, 32, 64, F16, 4, 3000)])
+def test_decode_q4_joins_of_unequal_rows(ops, h, hkv, d, dtype, rows, longest):
+    """One row of very many parts among short ones, and 127 to 147 pairs of one head each (the join's form goes by
+    the mean number of parts)."""
+    gen = torch.Generator().manual_seed(rows)
+    bs, nb = 16, 120
+    k, v = (torch.randn(nb * bs, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    cache = torch.zeros(ops.kv_cache_q4_shape(nb, hkv, bs, d), dtype=torch.uint8, device="cuda")
+    ops.kv_cache_update_q4(k.cuda(), v.cuda(), cache, torch.arange(nb * bs, device="cuda"))
+    kq, vq = R.read_q4(cache.cpu().numpy(), np.arange(nb * bs), dtype)
+    lens = torch.randint(1, 300, (rows,), generator=gen).numpy() if h != hkv else torch.randint(300, longest, (rows,), generator=gen).numpy()
+    lens[rows // 3] = longest
+    table = torch.randint(0, nb, (rows, -(-longest // bs)), generator=gen, dtype=torch.int32)
+    q = torch.randn(rows, h, d, generator=gen).to(dtype)
+    out, lse = torch.zeros(rows, h, d, dtype=dtype, device="cuda"), torch.zeros(h, rows, device="cuda")
+    ops.decode_splitkv_q4(q.cuda(), cache, table.cuda(), _i32(lens), scale=d ** -0.5, out=out, lse=lse)
+    o, l, t = R.f64(out), R.f64(lse), table.numpy()
+    for r in sorted({0, 1, rows // 3, rows - 1}):
+        p = np.arange(lens[r])
+        at = t[r, p // bs].astype(np.int64) * bs + p % bs
+        _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq[at], vq[at], d ** -0.5, dtype, (r, int(lens[r])))
