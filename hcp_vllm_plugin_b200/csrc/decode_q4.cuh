@@ -532,11 +532,25 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
             limit[nt][e] = now == -INFINITY ? -INFINITY : __fdividef(now + kRescaleThreshold, hs[nt][e]);
             l_run[nt][e] *= al;
             const int ea = static_cast<int>(__float_as_uint(al) >> 23);
+            // scales' exponents of the largest score's key, whose weight is 1 now
+            uint32_t top = 0u;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const uint32_t es = (__float_as_uint(vs[u][r][0]) >> 23) | (__float_as_uint(vs[u][r][NG - 1]) >> 23) << 16;
+                top = __vmaxu2(top, sc[u][nt][e + 2 * r] == mx ? es : 0u);
+              }
+#pragma unroll
+            for (int s = 4; s < 32; s <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, s));
 #pragma unroll
             for (int a = 0; a < NG; ++a) {
               vz[nt][a][e] *= al;
-              // the unit falls with the weights it stands for, by al's power of two; the rest of al is the sums'
-              const int ev = static_cast<int>(__float_as_uint(vinv[nt][a][e]) >> 23), to = max(1, min(ev + 127 - ea, kDq4UnitTop));
+              // the unit falls with the weights it stands for, by al's power of two; the rest of al is the sums'.
+              // With the first keys it comes to 2^-8 to 2^-9 of the largest score's s
+              const int ev = static_cast<int>(__float_as_uint(vinv[nt][a][e]) >> 23);
+              const int es = static_cast<int>(a == 0 ? top & 0xffffu : top >> 16);
+              const int to = max(1, min(old < now && old == -INFINITY ? 262 - es : ev + 127 - ea, kDq4UnitTop));
               const float f = ea == 0 ? 0.f : __uint_as_float(__float_as_uint(al) + (static_cast<uint32_t>(to - ev) << 23));
               vinv[nt][a][e] = __uint_as_float(static_cast<uint32_t>(to) << 23);
 #pragma unroll
