@@ -26,9 +26,10 @@
 //     key weighs, so a large value that nobody attends takes no bits from the others.
 //     Rounding p_j s_j to 11 bits is off by at most 2^-11 of each key's term, and by
 //     2^-33 of the largest p s where that is more (fp16's smallest numbers).  The terms'
-//     weights sum to one: an eighth of what rounding the result to bf16 may be off, as
-//     much as rounding it to fp16.  A second product for the rest would add 8 matrix
-//     instructions to a tile's 16.
+//     weights sum to one, so this is an eighth of what rounding the result to bf16 may be
+//     off, and is left there.  A result of fp16 or 32 bits would show it: for those
+//     (REST) what the rounding leaves is multiplied too, which takes each term to 2^-22 for
+//     8 matrix instructions more on a tile's 16 (33 ragged rows, D 64, fp16: 17.7 us for 17.1).
 //
 // Split: all rows' tiles of 16 keys, heads outermost in a row, form one line that
 // the warps cut into equal pieces, so any mix of lengths is even and nothing about
@@ -206,7 +207,7 @@ __device__ __forceinline__ void dq4_store8(const DecodeQ4Params& p, long long ro
   }
 }
 
-template <int D, bool F16, int NT>
+template <int D, bool F16, int NT, bool REST>
 __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
     decode_q4_kernel(const __grid_constant__ DecodeQ4Params p) {
   using L = Q4<D>;
@@ -582,6 +583,7 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
         }
       // ---- the weights of the second product, p_j s_j in units of 1 / vinv
       uint32_t bp[U][NT][NG][2];
+      uint32_t br[REST ? U : 1][NT][NG][2];  // what that rounding leaves
       uint32_t largest;
       auto weigh = [&] {
         largest = 0u;
@@ -597,6 +599,10 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
                 const float2 y = __fmul2_rn(__fmul2_rn(make_float2(pr[u][nt][2 * e], pr[u][nt][2 * e + 1]), unit),
                                             make_float2(vs[u][e][a], vs[u][e][a]));
                 bp[u][nt][a][e] = pack2<true>(y.x, y.y);
+                if constexpr (REST) {
+                  const float2 h = q4_up2<true>(bp[u][nt][a][e]);
+                  br[u][nt][a][e] = pack2<true>(y.x - h.x, y.y - h.y);
+                }
                 largest = q4_max2_f16(largest, bp[u][nt][a][e]);
               }
             }
@@ -652,13 +658,20 @@ __global__ void __launch_bounds__(kDq4Threads, dq4_ctas_per_sm(NT))
             vz[nt][a][1] = zv.y;
             bp[u][nt][a][0] = movmatrix_t(bp[u][nt][a][0]);
             bp[u][nt][a][1] = movmatrix_t(bp[u][nt][a][1]);
+            if constexpr (REST) {
+              br[u][nt][a][0] = movmatrix_t(br[u][nt][a][0]);
+              br[u][nt][a][1] = movmatrix_t(br[u][nt][a][1]);
+            }
           }
 #pragma unroll
           for (int i2 = 0; i2 < 4; ++i2) {
             uint32_t fa[4];  // dims 2p (row g) and 2p+1 (row g+8) of tokens 4t, 4t+2 and 4t+1, 4t+3
             q4_pairs(vwords[i2], consts, fa);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma16816<true>(o[nt][a][i2], fa, bp[u][nt][a][0], bp[u][nt][a][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              mma16816<true>(o[nt][a][i2], fa, bp[u][nt][a][0], bp[u][nt][a][1]);
+              if constexpr (REST) mma16816<true>(o[nt][a][i2], fa, br[u][nt][a][0], br[u][nt][a][1]);
+            }
           }
         }
     }

@@ -1054,23 +1054,23 @@ int launch_norm_rope(NormRopeParams p, int64_t tokens, int kind, cudaStream_t st
                 &norm_rope_kernel<D, F16, TAB32, kRopeCacheQ4, false>);
 }
 
-bool g_dq4_attr_done[2][2][2][64];
+bool g_dq4_attr_done[2][2][2][2][64];
 
-template <int D, bool F16, int NT>
-int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
+template <int D, bool F16, int NT, bool REST>
+int launch_decode_q4_kernels(const DecodeQ4Params& p, cudaStream_t st) {
   constexpr int smem = sizeof(Dq4Smem<D>);
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cuda_failed();
   {
     std::lock_guard<std::mutex> lk(g_attr_mu);
-    bool& done = g_dq4_attr_done[D == 128][F16][NT == 2][dev];
+    bool& done = g_dq4_attr_done[D == 128][F16][NT == 2][REST][dev];
     if (!done) {
-      if (cudaFuncSetAttribute(decode_q4_kernel<D, F16, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      if (cudaFuncSetAttribute(decode_q4_kernel<D, F16, NT, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return cuda_failed();
       done = true;
     }
   }
-  const int rc = launch_chained(decode_q4_kernel<D, F16, NT>, dim3(kDq4Sms * dq4_ctas_per_sm(NT)), kDq4Threads, smem, st, p);
+  const int rc = launch_chained(decode_q4_kernel<D, F16, NT, REST>, dim3(kDq4Sms * dq4_ctas_per_sm(NT)), kDq4Threads, smem, st, p);
   if (rc != HCP_OK) return rc;
   const int64_t pairs = static_cast<int64_t>(p.rows) * p.num_kv_heads;
   const int64_t parts = kDq4Sms * dq4_ctas_per_sm(NT) * kDq4Warps / pairs + 2;  // of a pair, were the rows alike
@@ -1088,6 +1088,14 @@ int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
 }
 
 constexpr float kLog2e = 1.4426950408889634f;
+
+template <int D, bool F16, int NT>
+int launch_decode_q4(const DecodeQ4Params& p, cudaStream_t st) {
+  // what rounding the weights leaves would show in a result of more than bf16's 8 bits
+  if constexpr (!F16)
+    if (p.out_dt == HCP_BF16) return launch_decode_q4_kernels<D, F16, NT, false>(p, st);
+  return launch_decode_q4_kernels<D, F16, NT, true>(p, st);
+}
 
 int validate_decode_q4(const hcp_decode_q4_args* a) {
   if (a == nullptr) return HCP_ERR_INVALID;

@@ -389,6 +389,9 @@ int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, int32_t blo
  *   kv_lens[r] <= 0: out 0, lse -inf.  A request outside the table (negative, say)
  *   marks a padding row: out and lse stay as they were.  Lengths are cut to
  *   block_table_width * block_size; a page outside the cache holds no keys.
+ * Scores and sums are held in 32 bits; a key's weight times its group's scale is
+ * rounded to 11 bits where out is bf16, to 22 elsewhere.  Scores that pass 32 bits
+ * (and keys past 2^104, whose partial sums do) give NaN.
  * Needs hcp_decode_q4_workspace_bytes(args) bytes of 16-byte aligned device
  * workspace (its contents need no preparation; calls that may overlap on the GPU
  * need their own).

@@ -26,7 +26,7 @@ def _i32(x):
 
 # ------------------------------------------------------------------ values of very different sizes
 
-def _check_by_weight(got, lse, q, k, v, scale, dtype, what):
+def _check_by_weight(got, lse, q, k, v, scale, dtype, what, rounded=1.08 * 2.0 ** -11):
     """One row against 64 bits, each key's share of the bar in proportion to its own weight.
 
     With p_j the softmax weights and top_j the largest |v| of key j's 64 dims: a score is off by at most
@@ -47,7 +47,7 @@ def _check_by_weight(got, lse, q, k, v, scale, dtype, what):
         top = np.repeat(np.abs(vh).reshape(n, -1, 64).max(-1), 64, axis=1)
         held = p @ top / total
         dx = 2.0 ** -17 * scale * (np.abs(q[i]) * np.abs(kh).max(0)).sum()
-        slack = held * (np.expm1(2 * dx) + 1.08 * 2.0 ** -11 + 2.0 ** -15 + n / 8 * 2.0 ** -23 + n * 2.0 ** -32)
+        slack = held * (np.expm1(2 * dx) + rounded + 2.0 ** -15 + n / 8 * 2.0 ** -23 + n * 2.0 ** -32)
         eps = 0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2
         bar = slack + eps * (np.abs(o) + slack) + (2.0 ** -25 if dtype == F16 else 0.0)
         assert (np.abs(got[i] - o) <= bar).all(), (what, i, np.max(np.abs(got[i] - o) / bar))
@@ -369,3 +369,26 @@ def test_decode_q4_joins_of_unequal_rows(ops, h, hkv, d, dtype, rows, longest):
         p = np.arange(lens[r])
         at = t[r, p // bs].astype(np.int64) * bs + p % bs
         _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq[at], vq[at], d ** -0.5, dtype, (r, int(lens[r])))
+
+
+# ------------------------------------------------------------------ results of more than 8 bits
+
+@pytest.mark.parametrize("h,hkv,d,dtype,kind", [(28, 4, 128, BF16, torch.float32), (32, 2, 128, BF16, torch.float32),
+                                                (14, 2, 64, F16, F16), (14, 2, 64, F16, torch.float32), (12, 1, 128, F16, F16)])
+@pytest.mark.parametrize("n", [2, 5, 40, 700])
+def test_decode_q4_weights_of_22_bits(ops, n, h, hkv, d, dtype, kind):
+    """Where the result is not rounded to bf16, a weight's second 11 bits are multiplied too: off by 1.08 * 2^-22 of
+    each term and not by 2^-11.  Small queries, so that the scores' own share of the bar is small."""
+    gen = torch.Generator().manual_seed(n + h)
+    rows, bs, nb = 6, 16, 44
+    k, v = (torch.randn(nb * bs, hkv, d, generator=gen).to(dtype) for _ in range(2))
+    cache = torch.zeros(ops.kv_cache_q4_shape(nb, hkv, bs, d), dtype=torch.uint8, device="cuda")
+    ops.kv_cache_update_q4(k.cuda(), v.cuda(), cache, torch.arange(nb * bs, device="cuda"))
+    kq, vq = R.read_q4(cache.cpu().numpy(), np.arange(n), dtype)
+    q = (torch.randn(rows, h, d, generator=gen) * 2.0 ** -6).to(dtype)
+    out, lse = torch.zeros(rows, h, d, dtype=kind, device="cuda"), torch.zeros(h, rows, device="cuda")
+    ops.decode_splitkv_q4(q.cuda(), cache, torch.arange(nb, dtype=torch.int32, device="cuda").view(1, nb), _i32([n] * rows),
+                          scale=d ** -0.5, out=out, lse=lse, token_req=_i32([0] * rows))
+    o, l = R.f64(out), R.f64(lse)
+    for r in range(rows):
+        _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq, vq, d ** -0.5, kind, (n, r), rounded=1.08 * 2.0 ** -22)
