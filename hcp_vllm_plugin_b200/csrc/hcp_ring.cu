@@ -953,6 +953,11 @@ bool overlap(Span a, Span b) {
   return at < a.row || at + b.row > a.stride;
 }
 
+// Whether a result stands exactly where its input does.
+bool in_place(const Span& out, const Span& in) {
+  return out.base == in.base && out.row == in.row && (out.rows <= 1 || out.stride == in.stride);
+}
+
 // A plan's blocks read the lengths, the list and the table's old entries while others write the results.
 bool plan_overlaps(const hcp_step_plan_args& a) {
   const int64_t reqs = 4 * static_cast<int64_t>(a.num_reqs), toks = a.num_tokens;
@@ -1123,6 +1128,12 @@ int validate_decode_q4(const hcp_decode_q4_args* a) {
     return HCP_ERR_UNSUPPORTED;
   if (a->token_req == nullptr && a->block_table_rows < a->q_rows) return HCP_ERR_INVALID;
   if (a->lse != nullptr && a->lse_stride < a->q_rows) return HCP_ERR_INVALID;
+  // rows end at different times: a result may replace its own query row, and nothing else that is read
+  const int elt = a->out_dtype == HCP_F32 ? 4 : 2;
+  const Span q{reinterpret_cast<uintptr_t>(a->q), a->q_rows, 2 * a->q_row_stride, 2 * row},
+      out{reinterpret_cast<uintptr_t>(a->out), a->q_rows, elt * a->out_row_stride, elt * row},
+      lse{reinterpret_cast<uintptr_t>(a->lse), a->lse != nullptr ? H : 0, 4 * a->lse_stride, 4 * a->q_rows};
+  if ((!in_place(out, q) && overlap(out, q)) || overlap(lse, q) || overlap(lse, out)) return HCP_ERR_INVALID;
   return HCP_OK;
 }
 
@@ -1172,8 +1183,7 @@ extern "C" int hcp_qk_norm_rope(const hcp_norm_rope_args* a, void* stream) {
   const Span q = rows(a->q, a->q_row_stride, q_row), k = rows(a->k, a->k_row_stride, kv_row),
              v = cached ? rows(a->v, a->v_row_stride, kv_row) : Span{}, qo = rows(a->q_out, a->q_out_row_stride, q_row),
              ko = rows(a->k_out, a->k_out_row_stride, kv_row);
-  auto own = [](const Span& out, const Span& in) { return out.base == in.base && (out.rows <= 1 || out.stride == in.stride); };
-  if ((!own(qo, q) && overlap(qo, q)) || (!own(ko, k) && overlap(ko, k)) || overlap(qo, k) || overlap(ko, q) ||
+  if ((!in_place(qo, q) && overlap(qo, q)) || (!in_place(ko, k) && overlap(ko, k)) || overlap(qo, k) || overlap(ko, q) ||
       overlap(qo, v) || overlap(ko, v) || overlap(qo, ko))
     return HCP_ERR_INVALID;
   NormRopeParams p;
@@ -1273,6 +1283,10 @@ extern "C" int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, 
   const int rc = validate_q4_rows(key, value, num_tokens, key_row_stride, value_row_stride, slot_mapping, kv_cache,
                                   num_blocks, block_size, num_kv_heads, head_dim, dtype);
   if (rc != HCP_OK || num_tokens == 0) return rc;
+  const int64_t row = 2 * static_cast<int64_t>(num_kv_heads) * head_dim;
+  if (overlap(Span{reinterpret_cast<uintptr_t>(key), num_tokens, 2 * key_row_stride, row},
+              Span{reinterpret_cast<uintptr_t>(value), num_tokens, 2 * value_row_stride, row}))
+    return HCP_ERR_INVALID;
   Q4GatherParams p;
   p.cache = static_cast<const uint8_t*>(kv_cache);
   p.slot_mapping = slot_mapping;

@@ -285,6 +285,8 @@ int hcp_kv_cache_gather(const void* kv_cache, int64_t num_blocks, int32_t block_
  *   block), kv_len p + 1.
  * Rows past the step's last token: position, slot and request -1, kv_len 0.
  * Only the new entries of block_table are written, so a call can be repeated.
+ * Blocks are only taken: to give a finished request's n blocks back, the caller
+ * writes them over the last n taken entries of free_blocks and lowers *free_head by n.
  * *missing_out: blocks that were needed and not given (list or row exhausted).
  * No output may share memory with an input or another output (HCP_ERR_INVALID):
  * lengths are advanced by a copy of seq_lens after the call.
@@ -369,7 +371,7 @@ int hcp_qk_norm_rope(const hcp_norm_rope_args* args, void* stream);
  *
  * hcp_kv_cache_update_q4 / hcp_kv_cache_gather_q4: as hcp_kv_cache_update /
  * hcp_kv_cache_gather, on it.  A slot named twice in one update holds a mixture
- * of its rows.
+ * of its rows; key and value of a gather may not share memory (HCP_ERR_INVALID).
  */
 int hcp_kv_cache_update_q4(const void* key, const void* value, int64_t num_tokens,
                            int64_t key_row_stride, int64_t value_row_stride,
@@ -391,7 +393,8 @@ int hcp_kv_cache_gather_q4(const void* kv_cache, int64_t num_blocks, int32_t blo
  *   block_table_width * block_size; a page outside the cache holds no keys.
  * Scores and sums are held in 32 bits; a key's weight times its group's scale is
  * rounded to 11 bits where out is bf16, to 22 elsewhere.  Scores that pass 32 bits
- * (and keys past 2^104, whose partial sums do) give NaN.
+ * give NaN; keys past 2^104, whose partial sums do, are outside the range.  out may
+ * be q itself; sharing any other memory with q or lse is refused (HCP_ERR_INVALID).
  * Needs hcp_decode_q4_workspace_bytes(args) bytes of 16-byte aligned device
  * workspace (its contents need no preparation; calls that may overlap on the GPU
  * need their own).

@@ -93,3 +93,17 @@ def test_decode_q4_scale_range(scale, taken):
     assert (C.load().hcp_decode_q4_workspace_bytes(ctypes.byref(a)) > 0) == taken
     if not taken:
         assert C.load().hcp_decode_q4_splitkv(ctypes.byref(a), None) == 1
+
+
+@pytest.mark.parametrize("over", [
+    dict(out=_addr(1) + 256), dict(out=_addr(1), out_dtype=C.HCP_F32), dict(out=_addr(1), out_row_stride=2 * 28 * 128),
+    dict(out=_addr(1) + 28 * 256 - 16), dict(lse=_addr(1)), dict(lse=_addr(5) + 1024), dict(out=_addr(1), lse=_addr(1))])
+def test_decode_q4_results_may_not_overlap(over):
+    """Pieces of a row end at different times: a result may replace its own query row, and nothing else that is read."""
+    assert C.load().hcp_decode_q4_splitkv(ctypes.byref(_args(C.HcpDecodeQ4Args, DECODE, over)), None) == 1
+
+
+@pytest.mark.parametrize("value", [0, 256, -16, 3 * 1024 + 1008])
+def test_gather_q4_results_may_not_overlap(value):
+    key = _addr(1)
+    assert C.load().hcp_kv_cache_gather_q4(_addr(4), 9, 16, 4, 128, _addr(3), 4, key, key + value, 512, 512, C.HCP_BF16, None) == 1

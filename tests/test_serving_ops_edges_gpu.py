@@ -392,3 +392,22 @@ def test_decode_q4_weights_of_22_bits(ops, n, h, hkv, d, dtype, kind):
     o, l = R.f64(out), R.f64(lse)
     for r in range(rows):
         _check_by_weight(o[r], l[:, r], R.f64(q[r]), kq, vq, d ** -0.5, kind, (n, r), rounded=1.08 * 2.0 ** -22)
+
+
+def test_decode_q4_in_place(ops):
+    """The result in the place of the queries: as with a result of its own, rows that are cut and joined among them."""
+    gen = torch.Generator().manual_seed(40)
+    rows, h, hkv, d, bs, nb = 7, 28, 4, 128, 16, 100
+    k, v = (torch.randn(nb * bs, hkv, d, generator=gen).to(BF16).cuda() for _ in range(2))
+    cache = torch.zeros(ops.kv_cache_q4_shape(nb, hkv, bs, d), dtype=torch.uint8, device="cuda")
+    ops.kv_cache_update_q4(k, v, cache, torch.arange(nb * bs, device="cuda"))
+    table = torch.randint(0, nb, (rows, 1200), generator=gen, dtype=torch.int32).cuda()
+    lens, qkv = _i32([19000, 1, 0, 700, 5000, 33, 16]), torch.randn(rows, (h + 2 * hkv) * d, generator=gen).to(BF16).cuda()
+    q = qkv[:, : h * d].view(rows, h, d)
+    out, lse = torch.zeros(rows, h, d, dtype=BF16, device="cuda"), torch.zeros(h, rows, device="cuda")
+    ops.decode_splitkv_q4(q, cache, table, lens, scale=0.1, out=out, lse=lse)
+    for _ in range(5):
+        buf, again = qkv.clone(), torch.zeros_like(lse)
+        mine = buf[:, : h * d].view(rows, h, d)
+        ops.decode_splitkv_q4(mine, cache, table, lens, scale=0.1, out=mine, lse=again)
+        assert torch.equal(mine, out) and torch.equal(again, lse) and torch.equal(buf[:, h * d:], qkv[:, h * d:])
