@@ -127,6 +127,7 @@ class HcpDecodeArgs(ctypes.Structure):
     ]
 
 
+# Of the next three ``csrc/front.cpp`` fills its own: these are for hosts without torch, and the tests.
 class HcpStepPlanArgs(ctypes.Structure):
     _fields_ = [
         ("context_lens", ctypes.c_void_p), ("new_lens", ctypes.c_void_p), ("pos_base", ctypes.c_void_p),

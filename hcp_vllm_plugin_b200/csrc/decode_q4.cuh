@@ -29,22 +29,25 @@
 //     weights sum to one, so this is an eighth of what rounding the result to bf16 may be
 //     off, and is left there.  A result of fp16 or 32 bits would show it: for those
 //     (REST) what the rounding leaves is multiplied too, which takes each term to 2^-22 for
-//     8 matrix instructions more on a tile's 16 (33 ragged rows, D 64, fp16: 17.7 us for 17.1).
+//     8 matrix instructions more on a tile's 16 (33 ragged rows, D 64, fp16: 17.6 us for 17.1).
 //
 // Split: all rows' tiles of 16 keys, heads outermost in a row, form one line that
-// the warps cut into equal pieces, so any mix of lengths is even and nothing about
-// the lengths has to be known on the host.  Every block sums the lengths itself.  A
+// the warps cut into equal pieces, so any mix of lengths is even in this kernel (the
+// join's form goes by the mean number of parts) and nothing about the lengths has to be
+// known on the host.  Every block sums the lengths itself.  A
 // warp works alone: its tiles come through a ring of asynchronous copies in shared
 // memory, two tiles a step.  A (row, KV head) that lies inside one piece is written
 // to out from the warp's registers; one that is cut leaves a partial (O, base, sum)
 // per piece in the workspace, and a second kernel, scheduled as the first runs out,
 // joins them in order.
 //
-// Measured (28 heads over 4, D 128, bf16; a replayed graph): 64 rows x 32768 keys 234 us =
-// 5.2 TB/s, 0.80 of the measured copy rate, with 288 instructions a tile on three warps a
-// scheduler as the bound (250 us with every page in L2 as well); 1 x 131072 keys 26 us; 16 rows of
-// up to 300 keys 11.6 us, latencies.  Four warps a scheduler leave 128 registers, too few for
-// two tiles a step (254 us); two leave latency (255 us).
+// Measured (28 heads over 4, D 128, bf16; a replayed graph): 64 rows x 32768 keys 239 us =
+// 5.1 TB/s, 0.78 of the measured copy rate (273 us in a long stream of calls, whose power lowers the
+// clock); 1 x 131072 keys 26.9 us; 16 rows of up to 300 keys 11.9 us, latencies.  DRAM is half busy and
+// the pages' place does not matter (as long with all of them in L2); of the issue slots 57 % are, with
+// 293 instructions a tile.  What bounds it is a step's chain of dependent instructions on three warps
+// a scheduler (the stalls are fixed latencies and busy pipes).  Four warps a scheduler leave 128
+// registers, too few for two tiles a step (20 us more); two cover less latency (20 us more).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -122,8 +125,9 @@ __device__ __forceinline__ uint32_t movmatrix_t(uint32_t a) {
   return d;
 }
 
-// Whole numbers of a word's nibble pairs (i, i + 4) as n - 8 in fp16, exact.  With a
-// nibble in mantissa bits 0-3 of 1024 the value is 1024 + n, in bits 4-7 it is
+// Whole numbers of a word's nibble pairs (i, i + 4) as n - 8 in fp16, exact, by the
+// published method of 4-bit weight kernels: bits put into the mantissa of a power of two.
+// With a nibble in mantissa bits 0-3 of 1024 the value is 1024 + n, in bits 4-7 it is
 // 1024 + 16 n: two pairs without a shift, the other two after one shift by 8.  The two
 // constants come in registers that the compiler cannot see through: as immediates
 // they would cost a move at every use (an instruction takes one immediate).

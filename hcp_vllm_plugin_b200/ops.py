@@ -471,6 +471,8 @@ def kv_plan_step(context_lens: torch.Tensor, new_lens: torch.Tensor, block_table
     of the step's buffers (the tokens past it are dropped, the rows past the
     last token are padding).  ``pos_base`` [R] int32: global position of each
     request's first cached token (a context-parallel chunk), 0 if not given.
+    Blocks are only taken: to give a finished request's n blocks back, write them
+    over the last n taken entries of free_blocks and lower free_head by n.
 
     free_head is not changed: the new head is in the result.  A call repeated on
     the same lengths writes the same entries.
@@ -546,6 +548,8 @@ def decode_splitkv_q4(q: torch.Tensor, kv_cache: torch.Tensor, block_table: torc
     pages are read on the GPU, so a captured call follows them.  Rows without
     keys get 0 and -inf; rows with a negative request are padding and stay as
     they were.  Peer keys in 16 bits are joined by :func:`decode_splitkv` and
-    :func:`merge_attn_states`.
+    :func:`merge_attn_states`: give ``out`` as float32 then, which holds the
+    weights to 22 bits (11 for a bf16 out).  ``out`` may be q itself; a
+    ``workspace`` of the caller's serves one call at a time.
     """
     C.front().decode_q4(q, kv_cache, block_table, kv_lens, scale, out, lse, token_req, workspace)

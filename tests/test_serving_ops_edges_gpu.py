@@ -411,3 +411,26 @@ def test_decode_q4_in_place(ops):
         mine = buf[:, : h * d].view(rows, h, d)
         ops.decode_splitkv_q4(mine, cache, table, lens, scale=0.1, out=mine, lse=again)
         assert torch.equal(mine, out) and torch.equal(again, lse) and torch.equal(buf[:, h * d:], qkv[:, h * d:])
+
+
+def test_blocks_given_back_are_taken_again(ops):
+    """A finished request's blocks, written over the last taken entries of the list with the head lowered, go to the
+    next requests; no block is ever held twice."""
+    gen = torch.Generator().manual_seed(41)
+    reqs, width, bs = 6, 5, 16
+    free = torch.randperm(18, generator=gen).int().cuda()
+    head = torch.zeros(1, dtype=torch.int32, device="cuda")
+    table, held = torch.full((reqs, width), -1, dtype=torch.int32, device="cuda"), np.zeros(reqs, np.int64)
+    for step in range(30):
+        new = np.minimum(torch.randint(0, 30, (reqs,), generator=gen).numpy(), 45 - held)
+        plan = ops.kv_plan_step(_i32(held), _i32(new), table, free, head, block_size=bs, num_tokens=200)
+        assert plan.missing.item() == 0
+        held, head = held + new, plan.free_head.clone()
+        mine = [table[i, : -(-int(c) // bs)].tolist() for i, c in enumerate(held)]
+        flat = sum(mine, [])
+        assert len(set(flat)) == len(flat) == int(head) and sorted(flat + free[int(head):].tolist()) == list(range(18))
+        for i in np.flatnonzero(held >= 40):
+            n = len(mine[i])
+            free[int(head) - n: int(head)] = _i32(mine[i])
+            head -= n
+            held[i] = 0
