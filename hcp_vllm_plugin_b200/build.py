@@ -12,6 +12,7 @@ where there is no torch.
 
 from __future__ import annotations
 
+import glob
 import os
 import shutil
 import subprocess
@@ -24,7 +25,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libhcp_ring.so")
 SOURCES = [os.path.join(CSRC, "hcp_ring.cu")]
 HEADER = os.path.join(ROOT, "include", "hcp_ring.h")
-DEPS = SOURCES + [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cu", ".cuh"))] + [HEADER]
+DEPS = SOURCES + sorted(glob.glob(os.path.join(CSRC, "*.cuh"))) + [HEADER]
 FRONT = os.path.join(HERE, "_hcp_front.so")
 FRONT_SOURCE = os.path.join(CSRC, "front.cpp")
 

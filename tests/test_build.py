@@ -56,3 +56,15 @@ def test_a_front_end_built_for_another_torch_is_refused(monkeypatch):
     monkeypatch.setattr(B, "front_target", lambda: "torch 0.0.1, another Python")
     with pytest.raises(_capi.HcpError, match="built for torch"):
         _capi.front()
+
+
+def test_an_installed_package_without_sources_loads_its_modules(tmp_path):
+    """Loading asks the build what the module has to be for; that needs no source files."""
+    import os
+    import shutil
+    import subprocess
+    home = tmp_path / "hcp_vllm_plugin_b200"
+    shutil.copytree(os.path.dirname(B.__file__), home, ignore=shutil.ignore_patterns("csrc", "__pycache__", "*.tmp"))
+    r = subprocess.run([sys.executable, "-c", "from hcp_vllm_plugin_b200 import _capi; print(_capi.front().__name__)"],
+                       cwd=tmp_path, env={**os.environ, "PYTHONPATH": str(tmp_path)}, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "_hcp_front" in r.stdout, r.stderr[-800:]
